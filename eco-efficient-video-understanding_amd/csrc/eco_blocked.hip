@@ -1034,11 +1034,11 @@ __global__ __launch_bounds__(256, 2) void convb_spanp_kernel(const ConvBArgs a, 
           if (stores) { wait_newest_behind_stores(newest, stores); stores = 0; }
           else wait_newest(newest);
           // Dynamic items: the next item's ticket is drawn here, at the first tap of this item's last group -- the last moment
-          // that keeps the next item's span and first weights in flight under this group -- by wave 0 on the scalar unit
-          // (s_atomic_add: ~600 cycles, nothing in the vector memory counter; the other waves meet it at the barrier below).
+          // that keeps the next item's span and first weights in flight under this group -- by wave 0
+          // (a device-scope add by one lane; the other waves meet it at the barrier below).
           // Drawn an item ahead, every workgroup had reserved its second item before any work was done and res4 (1.5 items
-          // per workgroup) ran 28 % slower than with static shares; the compiler's own returning atomic is waited for with
-          // vmcnt(0) where it is issued.
+          // per workgroup) ran 28 % slower than with static shares; the returned ticket is waited for with
+          // vmcnt(0), the wave's newest weights with it.
           if (xx == 0 && y == 0 && last_group && dynamic && wave == 0) {
 #ifdef ECO_EMU
             if (tid == 0)

@@ -407,16 +407,16 @@ __device__ __forceinline__ unsigned counter_fetch_add(unsigned* p, unsigned v) {
   return __hip_atomic_fetch_add(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 #endif
 }
-// The same for a whole wave at once, on the scalar unit (s_atomic_add, returning form; p wave-uniform): ~600 cycles round
-// trip for a wave on its own (tools/ubench/satomic_check.hip), nothing in the vector memory counter.  The wait is part of
-// the statement: the compiler must not copy the result register before the value is in it.
+// The same for a whole wave at once (p wave-uniform): lane 0 adds through the vector memory path and every lane gets its
+// ticket.  The compiler waits for the returned value (vmcnt(0)) where it is read: LDS-DMA pieces that the wave has in
+// flight are waited for as well, so a caller that counts its own pieces finds fewer outstanding than it assumes, never more.
 __device__ __forceinline__ unsigned counter_draw_wave(unsigned* p) {
 #ifdef ECO_EMU
   return __atomic_fetch_add(p, 1u, __ATOMIC_SEQ_CST);   // (called by one fiber of the workgroup)
 #else
-  unsigned t = 1u;
-  asm volatile("s_atomic_add %0, %1, 0x0 glc\n\ts_waitcnt lgkmcnt(0)" : "+s"(t) : "s"(p) : "memory");
-  return t;
+  unsigned t = 0u;
+  if ((threadIdx.x & 63u) == 0u) t = __hip_atomic_fetch_add(p, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  return (unsigned)__builtin_amdgcn_readfirstlane((int)t);
 #endif
 }
 __device__ __forceinline__ void counter_store(unsigned* p, unsigned v) {

@@ -218,7 +218,7 @@ __global__ __launch_bounds__(256, 2) void stemb_kernel(const StemBArgs a) {
   const int cblocks = a.cout / 8;
 
   // Patches: the first is blockIdx.x; after it either every gridDim.x-th, or -- dynamic -- the next one nobody has taken
-  // (patch gridDim.x + ticket), drawn by wave 0 on the scalar unit when the patch's loads are about to be issued (two patches
+  // (patch gridDim.x + ticket), drawn by wave 0 when the patch's loads are about to be issued (two patches
   // ahead of its reduction) and passed through LDS behind a barrier the loop has anyway.  The two workgroups of a CU do not
   // run at the same speed (the instruction arbiter prefers the older wave): with equal shares block b finished its 56
   // patches in 421 us and block b + 256 in 510 us (tools/exp/clock_probe2.sh).

@@ -29,7 +29,7 @@ def test_switched_forms_match_the_oracle(env, args):
 
 
 # ---- the same switches on the hardware (the forms above had only ever run under the emulator, which MODELS
-# buffer_load ... lds zero-fill, s_atomic_add and v_permlane32_swap but cannot confirm them).  Each setting runs the hip-backend
+# buffer_load ... lds zero-fill, the shared work counters and v_permlane32_swap but cannot confirm them).  Each setting runs the hip-backend
 # kernel tests it affects -- the small cases AND the real ECO layer geometries (tests/test_blocked.py ECO_CONVS_B) -- in a child
 # process on the GPU box.
 GPU_CASES = [

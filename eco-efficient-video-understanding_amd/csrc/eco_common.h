@@ -22,6 +22,13 @@ inline int check_launch(const char* what) {
 
 inline long ceil_div(long a, long b) { return (a + b - 1) / b; }
 
+// Whether `rows` >= 1 rows of `width` elements, `stride` >= 0 elements apart, end below 2^58 elements: byte offsets into them
+// (of types up to 8 bytes) then fit 64-bit arithmetic.
+inline bool extent_fits(long rows, long stride, long width) {
+  long v = 0;
+  return !__builtin_mul_overflow(rows - 1, stride, &v) && !__builtin_add_overflow(v, width, &v) && v <= (1l << 58);
+}
+
 // Work-counter slot (0 .. 255) of a dynamic-share launch on `stream`, or -1 (the launch then takes static shares):
 // eager launches get ONE slot per stream -- launches of a stream run in order, and a launch's last workgroup leaves the
 // slot zero for the next -- for up to 64 distinct streams; launches recorded by a stream capture take slots 64 .. 255 in

@@ -54,7 +54,7 @@ class TorchAllocator:
     def empty(self, nelems: int, dtype=np.float32):
         # uint16 = raw bf16 bits (the blocked bf16 path); torch has no uint16 arithmetic, the buffer is int16
         tdt = {np.dtype(np.float32): self.torch.float32, np.dtype(np.int32): self.torch.int32,
-               np.dtype(np.uint16): self.torch.int16}[np.dtype(dtype)]
+               np.dtype(np.uint16): self.torch.int16, np.dtype(np.int8): self.torch.int8}[np.dtype(dtype)]
         return self.torch.empty(max(int(nelems), 1), dtype=tdt, device=self.device)
 
     @staticmethod

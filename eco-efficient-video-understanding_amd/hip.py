@@ -21,9 +21,12 @@ ECO_ERR_INVALID = -1
 ECO_ERR_RUNTIME = -2
 POOL_MAX = 0
 POOL_AVE = 1
-ABI_VERSION = 19
+ABI_VERSION = 20
 MAX_SEG = 3   # ECO_MAX_SEG: extra output segments of a sibling launch
+DT_F32 = 0     # ECO_DT_*: element types of the channels-last operators
 DT_BF16 = 1
+ACT_NONE, ACT_RELU, ACT_SILU = 0, 1, 2   # ECO_ACT_*
+I8_MAX_K = 131071
 
 _i32x3 = C.c_int32 * 3
 
@@ -62,6 +65,17 @@ class WGemmPlan(C.Structure):
                 ("tw", C.c_int32), ("kd", C.c_int32), ("points", C.c_int32), ("bm", C.c_int32), ("bn", C.c_int32),
                 ("nstages", C.c_int32), ("ksplit", C.c_int32), ("mblocks", C.c_int32), ("bmp", C.c_int32),
                 ("q", C.c_int64), ("u_elems", C.c_int64), ("v_elems", C.c_int64), ("m_elems", C.c_int64)]
+
+
+class GroupNormPlan(C.Structure):
+    _fields_ = [("n", C.c_int64), ("s", C.c_int64), ("c", C.c_int32), ("groups", C.c_int32), ("dt", C.c_int32),
+                ("num_cu", C.c_int32), ("chunks", C.c_int32), ("reserved", C.c_int32), ("ws_bytes", C.c_int64)]
+
+
+class InnerProductI8Plan(C.Structure):
+    _fields_ = [("m", C.c_int64), ("n", C.c_int32), ("k", C.c_int32), ("dt", C.c_int32), ("num_cu", C.c_int32),
+                ("bm", C.c_int32), ("bn", C.c_int32), ("ksplit", C.c_int32), ("reserved", C.c_int32),
+                ("ws_bytes", C.c_int64)]
 
 
 class View(C.Structure):
@@ -273,6 +287,18 @@ _SIGNATURES = {
     "eco_global_avgpool_fc_b_forward": (C.c_int, [C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64,
                                                   C.c_int64, C.c_int64, C.c_int64, C.c_int64, C.c_int64, C.c_int,
                                                   C.c_void_p]),
+    "eco_group_norm_plan_create": (C.c_int, [C.c_int64, C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_int32,
+                                             C.POINTER(GroupNormPlan)]),
+    "eco_group_norm_forward": (C.c_int, [C.POINTER(GroupNormPlan), C.c_void_p, C.c_int64, C.c_int64, C.c_void_p, C.c_void_p,
+                                         C.c_void_p, C.c_float, C.c_int32, C.c_void_p, C.c_int64, C.c_int64, C.c_void_p,
+                                         C.c_void_p]),
+    "eco_quant_rows_forward": (C.c_int, [C.c_void_p, C.c_int32, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64,
+                                         C.c_int64, C.c_void_p]),
+    "eco_inner_product_i8_plan_create": (C.c_int, [C.c_int64, C.c_int64, C.c_int64, C.c_int32, C.c_int32,
+                                                   C.POINTER(InnerProductI8Plan)]),
+    "eco_inner_product_i8_forward": (C.c_int, [C.POINTER(InnerProductI8Plan), C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p,
+                                               C.c_int64, C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_int64,
+                                               C.c_void_p, C.c_void_p]),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
@@ -576,6 +602,38 @@ class EcoLib:
                              stream=None) -> None:
         self._check(self._dll.eco_softmax_loss_forward(x, label, out, outer, c, inner, bool(normalize),
                                                        ignore_label is not None, ignore_label or 0, stream))
+
+    # -- channels-last pointwise block: group norm + activation, rows to 8-bit integers, 8-bit product ----------
+    def group_norm_plan(self, n: int, s: int, c: int, groups: int, dt: int, num_cu: Optional[int] = None) -> "GroupNormPlan":
+        """x[n][s][c] (channels last), statistics over c/groups channels and an image's positions; dt = DT_F32 | DT_BF16."""
+        p = GroupNormPlan()
+        self._check(self._dll.eco_group_norm_plan_create(n, s, c, groups, int(dt), 0 if num_cu is None else int(num_cu),
+                                                         C.byref(p)))
+        return p
+
+    def group_norm_forward(self, p: "GroupNormPlan", x, gamma, beta, y, eps: float = 1e-5, act: int = ACT_NONE, lengths=None,
+                           x_strides=(0, 0), y_strides=(0, 0), workspace=None, stream=None) -> None:
+        """y = act((x - mean) / sqrt(var + eps) * gamma + beta); *_strides = (image, row) in elements, 0 = dense; lengths:
+        device int32[n] of valid positions (the others are neither read nor written); workspace: p.ws_bytes bytes."""
+        self._check(self._dll.eco_group_norm_forward(C.byref(p), x, x_strides[0], x_strides[1], lengths, gamma, beta,
+                                                     float(eps), int(act), y, y_strides[0], y_strides[1], workspace, stream))
+
+    def quant_rows_forward(self, x, dt: int, q, scale, m: int, k: int, ldx: int = 0, ldq: int = 0, stream=None) -> None:
+        """q[m][k] = nearest integers to 127 x / max|row|, scale[m] = max|row| / 127 (rows ldx elements / ldq bytes apart)."""
+        self._check(self._dll.eco_quant_rows_forward(x, int(dt), ldx, q, ldq, scale, m, k, stream))
+
+    def inner_product_i8_plan(self, m: int, n: int, k: int, dt: int, num_cu: Optional[int] = None) -> "InnerProductI8Plan":
+        """y[m][n] of type dt from int8 x[m][k] and w[n][k]."""
+        p = InnerProductI8Plan()
+        self._check(self._dll.eco_inner_product_i8_plan_create(m, n, k, int(dt), 0 if num_cu is None else int(num_cu),
+                                                               C.byref(p)))
+        return p
+
+    def inner_product_i8_forward(self, p: "InnerProductI8Plan", x, sx, w, sw, bias, y, act: int = ACT_NONE, ldx: int = 0,
+                                 ldw: int = 0, ldy: int = 0, workspace=None, stream=None) -> None:
+        """y = act(sum x w * sx[row] * sw[channel] + bias); bias may be None; workspace: p.ws_bytes bytes."""
+        self._check(self._dll.eco_inner_product_i8_forward(C.byref(p), x, ldx, sx, w, ldw, sw, bias, int(act), y, ldy,
+                                                           workspace, stream))
 
 
 _PKG_DIR = os.path.dirname(os.path.abspath(__file__))

@@ -20,6 +20,8 @@
 #include <utility>
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef int i32x16 __attribute__((ext_vector_type(16)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 namespace eco {
 
@@ -45,6 +47,25 @@ __device__ __forceinline__ f32x16 mfma_32x32x16_bf16(uint4 a, uint4 b, f32x16 c)
 #else
   typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+#endif
+}
+
+// D(32x32) += A(32x32) * B(32x32), int8 in / int32 accumulate (v_mfma_i32_32x32x32_i8): lane l supplies sixteen consecutive k of
+// row / column l&31, A[l&31][16*(l>>5) + e]; C/D as the f32 form.  Any permutation of k that A and B share gives the same sum.
+__device__ __forceinline__ i32x16 mfma_32x32x32_i8(uint4 a, uint4 b, i32x16 c) {
+#ifdef ECO_EMU
+  return emu::mfma_i32_32x32x32_i8(a, b, c);
+#else
+  return __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b), c, 0, 0, 0);
+#endif
+}
+// D(16x16) += A(16x64) * B(64x16) (v_mfma_i32_16x16x64_i8): lane l supplies A[l&15][16*(l>>4) + e]; reg r of the result is
+// D[4*(l>>4) + r][l&15].
+__device__ __forceinline__ i32x4 mfma_16x16x64_i8(uint4 a, uint4 b, i32x4 c) {
+#ifdef ECO_EMU
+  return emu::mfma_i32_16x16x64_i8(a, b, c);
+#else
+  return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b), c, 0, 0, 0);
 #endif
 }
 

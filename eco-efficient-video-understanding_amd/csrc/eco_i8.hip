@@ -71,11 +71,16 @@ struct I8Args {
   const float* sw;
   const float* bias;
   void* y;
+  int* part;               // [ksplit][m][n] partial sums (ksplit > 1)
   long ldx, ldw, ldy;
   long m;
   int n, k, act;
+  int vec;                 // y's rows allow 16-byte stores of eight (f32: four) consecutive channels
+  int ksplit, nstages;     // slices; 64-byte stages of the whole sum
+  int tiles_m, tiles_n;
 };
 
+// (int -> fp32 rounds once; the products and the sum once each)
 __device__ __forceinline__ float i8_epilogue(int acc, float sx, float sw, float bias, int act) {
   float v = (float)acc * sx * sw + bias;
   if (act == ECO_ACT_RELU) v = v < 0.0f ? 0.0f : v;
@@ -85,24 +90,366 @@ __device__ __forceinline__ float i8_epilogue(int acc, float sx, float sw, float 
 __device__ __forceinline__ void i8_store(float* p, float v) { st(p, v); }
 __device__ __forceinline__ void i8_store(unsigned short* p, float v) { st(p, (unsigned short)f32_to_bf16_bits(v)); }
 
-// One thread per output.
+// Sixteen bytes of a row from byte `at` on (at < k): an unaligned 16-byte load, or -- where the row ends inside -- its last bytes
+// one by one and zeros.  Nothing outside the row is read.
+__device__ __forceinline__ uint4 i8_chunk(const signed char* row, int at, int k) {
+  uint4 q = make_uint4(0u, 0u, 0u, 0u);
+  if (at + 16 <= k) {
+#ifdef ECO_EMU
+    if (!emu::check_access(row + at, 16, false)) return q;
+#endif
+    __builtin_memcpy(&q, row + at, 16);
+  } else if (at < k) {
+    unsigned u[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+      if (at + e < k) u[e >> 2] |= (unsigned)(unsigned char)ld(row + at + e) << (8 * (e & 3));
+    q = make_uint4(u[0], u[1], u[2], u[3]);
+  }
+  return q;
+}
+template <bool FAST>
+__device__ __forceinline__ uint4 i8_chunk_of(const signed char* row, int at, int k) {
+  if constexpr (FAST) return at < k ? ld((const uint4*)(row + at)) : make_uint4(0u, 0u, 0u, 0u);
+  else return i8_chunk(row, at, k);
+}
+
+// ---- few tokens (m <= 32): bound by the weights' bytes ----------------------------------------------------------------------
+// A workgroup takes 16 output channels; its eight waves share the sum in units of 128 bytes.  Weights go from memory straight into
+// the matrix instruction's registers (16 rows x 64 bytes each), the tokens' bytes come from the caches in the same order of k,
+// and the waves' partial sums meet in LDS: one launch, no workspace.  Four units (eight 16-byte loads a lane) are in flight per
+// wave.
+constexpr int kTokWaves = 8, kTokUnit = 128, kTokFlight = 4;
+template <int MT, bool FAST, typename T>
+__global__ __launch_bounds__(512) void i8_token_kernel(const I8Args a) {
+  __shared__ i32x4 red[kTokWaves][MT][kWave];
+  const int lane = lane_id(), wave = uniform((int)(threadIdx.x >> 6));
+  const int n0 = (int)blockIdx.x * 16;
+  const int r16 = lane & 15, kc = (lane >> 4) * 16;
+  const bool w_ok = n0 + r16 < a.n;
+  const signed char* wrow = a.w + (long)(w_ok ? n0 + r16 : 0) * a.ldw;
+  const signed char* xrow[MT];
+  bool x_ok[MT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t) {
+    x_ok[t] = t * 16 + r16 < a.m;
+    xrow[t] = a.x + (long)(x_ok[t] ? t * 16 + r16 : 0) * a.ldx;
+  }
+  i32x4 acc[MT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t) acc[t] = i32x4{0, 0, 0, 0};
+  const int units = (a.k + kTokUnit - 1) / kTokUnit;
+  for (int u0 = wave; u0 < units; u0 += kTokWaves * kTokFlight) {
+    uint4 wq[kTokFlight][2], xq[kTokFlight][2][MT];
+#pragma unroll
+    for (int f = 0; f < kTokFlight; ++f)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int at = (u0 + f * kTokWaves) * kTokUnit + h * 64 + kc;     // (past the end: zeros)
+        wq[f][h] = w_ok ? i8_chunk_of<FAST>(wrow, at, a.k) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+        for (int t = 0; t < MT; ++t) xq[f][h][t] = x_ok[t] ? i8_chunk_of<FAST>(xrow[t], at, a.k) : make_uint4(0u, 0u, 0u, 0u);
+      }
+#pragma unroll
+    for (int f = 0; f < kTokFlight; ++f)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int t = 0; t < MT; ++t) acc[t] = mfma_16x16x64_i8(wq[f][h], xq[f][h][t], acc[t]);
+  }
+#pragma unroll
+  for (int t = 0; t < MT; ++t) red[wave][t][lane] = acc[t];
+  __syncthreads();
+  const int tid = (int)threadIdx.x;
+  if (tid < MT * 256) {       // one output each: channel fastest
+    const int t = tid >> 8, tok = (tid >> 4) & 15, ch = tid & 15;
+    const int from = (ch >> 2) * 16 + tok;
+    int sum = 0;
+#pragma unroll
+    for (int v = 0; v < kTokWaves; ++v) sum += red[v][t][from][ch & 3];
+    const int i = t * 16 + tok, j = n0 + ch;
+    if (i < a.m && j < a.n)
+      i8_store((T*)a.y + (long)i * a.ldy + j,
+               i8_epilogue(sum, ld(a.sx + i), ld(a.sw + j), a.bias ? ld(a.bias + j) : 0.0f, a.act));
+  }
+}
+
+// ---- tiles on the matrix cores -------------------------------------------------------------------------------------------------
+// A workgroup of four waves takes BN output channels x BM rows, each wave WN x WM of them as 32x32 products
+// (D's rows are channels, so that a lane ends up with consecutive channels of one row of y).  Both operands pass through LDS in
+// stages of 64 bytes of k, rows 64 bytes apart, the four 16-byte chunks of row r stored in the order c ^ ((r >> 1) & 3): eight
+// lanes that read a fragment then touch all 32 banks once.
+//   FAST  (rows on 16-byte boundaries, k a multiple of 16): LDS-DMA into NBUF buffers, NBUF - 1 stages ahead; a buffer is refilled
+//         behind the barrier in the middle of its own stage, when every wave has its last fragments in registers
+//   else  any alignment: through registers, one stage ahead, two buffers
+template <int BM, int BN, int WM, int WN, int NBUF, bool FAST, typename T>
+__global__ __launch_bounds__(256, (BM * BN > 128 * 128) ? 1 : 2) void i8_tile_kernel(const I8Args a) {
+  constexpr int TM = WM / 32, TN = WN / 32;              // 32x32 products of a wave
+  constexpr int WAVES_N = BN / WN;
+  static_assert((BM / WM) * (BN / WN) == 4, "four waves");
+  constexpr int STAGE = (BM + BN) * 4;                   // 16-byte vectors of a stage: BN rows of w, then BM rows of x
+  constexpr int PW = BN / 16 / 4, PX = BM / 16 / 4;      // DMA pieces (16 rows x 64 bytes) of a wave per stage
+  ECO_DYNAMIC_LDS(lds_f);
+  uint4* const lds = (uint4*)lds_f;
+  const int tid = (int)threadIdx.x, lane = lane_id(), wave = uniform(tid >> 6);
+  const int half = lane >> 5, l31 = lane & 31;
+
+  // XCD-contiguous tile numbers, then groups of eight row tiles by all channel tiles: the tiles that run side by side on an XCD
+  // share their operands through its L2
+  const int tiles = a.tiles_m * a.tiles_n;
+  const int id = xcd_remap((int)blockIdx.x, tiles * a.ksplit);
+  const int slice = id / tiles, tile = id - slice * tiles;
+  const int per = 8 * a.tiles_n, grp = tile / per, first = grp * 8;
+  const int gm = a.tiles_m - first < 8 ? a.tiles_m - first : 8;
+  const int in = tile - grp * per;
+  const long m0 = (long)(first + in % gm) * BM;
+  const int n0 = (in / gm) * BN;
+  const int s_begin = (int)((long)a.nstages * slice / a.ksplit), s_end = (int)((long)a.nstages * (slice + 1) / a.ksplit);
+  const int ns = s_end - s_begin;
+
+  const int wn = (wave % WAVES_N) * WN, wm = (wave / WAVES_N) * WM;
+  i32x16 acc[TN][TM];
+#pragma unroll
+  for (int i = 0; i < TN; ++i)
+#pragma unroll
+    for (int j = 0; j < TM; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0;
+
+  uint4 wf[2][TN], xf[2][TM];
+  auto read_frags = [&](int slot, const uint4* buf, int ks) {
+    const int c = (2 * ks + half) ^ ((l31 >> 1) & 3);
+#pragma unroll
+    for (int i = 0; i < TN; ++i) wf[slot][i] = buf[(wn + 32 * i + l31) * 4 + c];
+#pragma unroll
+    for (int j = 0; j < TM; ++j) xf[slot][j] = buf[(BN + wm + 32 * j + l31) * 4 + c];
+  };
+  auto multiply = [&](int slot) {
+#pragma unroll
+    for (int i = 0; i < TN; ++i)
+#pragma unroll
+      for (int j = 0; j < TM; ++j) acc[i][j] = mfma_32x32x32_i8(wf[slot][i], xf[slot][j], acc[i][j]);
+  };
+
+  if constexpr (FAST) {
+    // descriptors from the tile's first row to the operand's end: rows behind the last one read zeros
+    const long wext = (long)(a.n - n0 - 1) * a.ldw + a.k, xext = (a.m - m0 - 1) * a.ldx + a.k;
+    const BufRsrc rw = make_buf_rsrc(a.w + (long)n0 * a.ldw, (unsigned)(wext < 0x7fffffffl ? wext : 0x7fffffffl));
+    const BufRsrc rx = make_buf_rsrc(a.x + m0 * a.ldx, (unsigned)(xext < 0x7fffffffl ? xext : 0x7fffffffl));
+#ifndef ECO_EMU
+    // (descriptor words written by readfirstlane: five wait states before a memory instruction inside asm may read them)
+    asm volatile("s_nop 4" ::"s"(rw), "s"(rx));
+#endif
+    const int prow = lane >> 2, pchunk = (lane & 3) ^ ((prow >> 1) & 3);
+    const unsigned vw = (unsigned)((long)prow * a.ldw + pchunk * 16), vx = (unsigned)((long)prow * a.ldx + pchunk * 16);
+    const unsigned ldw16 = (unsigned)(16 * a.ldw), ldx16 = (unsigned)(16 * a.ldx);
+    auto issue = [&](int s) {           // stage s of this slice -> buffer s % NBUF
+      const int k0 = (s_begin + s) * 64;
+      const bool in_k = k0 + pchunk * 16 < a.k;            // (the last stage's chunks behind k: zeros)
+      const unsigned ow = in_k ? vw : kBufOob, ox = in_k ? vx : kBufOob;
+      uint4* const buf = lds + (s % NBUF) * STAGE;
+#pragma unroll
+      for (int p = 0; p < PW; ++p) {
+        const int piece = p * 4 + wave;
+        glds16_buf(rw, ow, (unsigned)k0 + (unsigned)piece * ldw16, buf + piece * 64);
+      }
+#pragma unroll
+      for (int p = 0; p < PX; ++p) {
+        const int piece = p * 4 + wave;
+        glds16_buf(rx, ox, (unsigned)k0 + (unsigned)piece * ldx16, buf + BN * 4 + piece * 64);
+      }
+    };
+    auto wait_stage = [&](int newer) {  // this wave's pieces of all but the newest `newer` stages have landed
+      if (newer >= 2 && NBUF > 3) wait_dma_all_but<2 * (PW + PX)>();
+      else if (newer >= 1) wait_dma_all_but<PW + PX>();
+      else wait_dma_all_but<0>();
+    };
+    for (int s = 0; s < NBUF - 1 && s < ns; ++s) issue(s);
+    {
+      const int newer = (ns < NBUF - 1 ? ns : NBUF - 1) - 1;
+      wait_stage(newer);
+    }
+    wg_barrier_nodrain();
+    // one more stage ahead than the buffers behind the barrier above: buffer NBUF - 1 is still empty
+    if (NBUF - 1 < ns) issue(NBUF - 1);
+    read_frags(0, lds, 0);
+    for (int s = 0; s < ns; ++s) {
+      read_frags(1, lds + (s % NBUF) * STAGE, 1);
+      multiply(0);
+      if (s + 1 < ns) {
+        // stages s+1 .. min(s+NBUF-1, ns-1) are in flight: s+1 must have landed
+        const int newer = (ns - 1 < s + NBUF - 1 ? ns - 1 : s + NBUF - 1) - (s + 1);
+        wait_stage(newer);
+#ifndef ECO_EMU
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // this wave's fragments of stage s are in registers
+#endif
+        wg_barrier_nodrain();
+        if (s + NBUF < ns) issue(s + NBUF);                  // into the buffer that stage s leaves
+        read_frags(0, lds + ((s + 1) % NBUF) * STAGE, 0);
+      }
+      multiply(1);
+    }
+  } else {
+    constexpr int CH = STAGE / 256;       // chunks of a thread per stage
+    uint4 q[CH];
+    auto fetch = [&](int s) {
+      const int k0 = (s_begin + s) * 64;
+#pragma unroll
+      for (int p = 0; p < CH; ++p) {
+        const int id4 = p * 256 + tid, row = id4 >> 2, at = k0 + (id4 & 3) * 16;
+        q[p] = make_uint4(0u, 0u, 0u, 0u);
+        if (row < BN) { if (n0 + row < a.n) q[p] = i8_chunk(a.w + (long)(n0 + row) * a.ldw, at, a.k); }
+        else if (m0 + row - BN < a.m) q[p] = i8_chunk(a.x + (m0 + row - BN) * a.ldx, at, a.k);
+      }
+    };
+    auto put = [&](int s) {
+#pragma unroll
+      for (int p = 0; p < CH; ++p) {
+        const int id4 = p * 256 + tid, row = id4 >> 2;
+        lds[(s & 1) * STAGE + row * 4 + ((id4 & 3) ^ ((row >> 1) & 3))] = q[p];
+      }
+    };
+    fetch(0);
+    put(0);
+    __syncthreads();
+    for (int s = 0; s < ns; ++s) {
+      if (s + 1 < ns) fetch(s + 1);
+      read_frags(0, lds + (s & 1) * STAGE, 0);
+      read_frags(1, lds + (s & 1) * STAGE, 1);
+      multiply(0);
+      multiply(1);
+      if (s + 1 < ns) put(s + 1);
+      __syncthreads();
+    }
+  }
+
+  // ---- epilogue: a lane holds row m0 + wm + 32 j + l31 and channels 8 q + 4 half + {0..3}, q = 0..3, of each 32-channel block
+  if (a.ksplit > 1) {
+#pragma unroll
+    for (int j = 0; j < TM; ++j) {
+      const long row = m0 + wm + 32 * j + l31;
+      if (row < a.m) {
+        int* const to = a.part + ((long)slice * a.m + row) * a.n;
+#pragma unroll
+        for (int i = 0; i < TN; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int ch = n0 + wn + 32 * i + (r & 3) + 8 * (r >> 2) + 4 * half;
+            if (ch < a.n) st(to + ch, acc[i][j][r]);
+          }
+      }
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < TN; ++i) {
+    float sw[16], bias[16];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int ch = n0 + wn + 32 * i + (r & 3) + 8 * (r >> 2) + 4 * half;
+      sw[r] = ch < a.n ? ld(a.sw + ch) : 0.0f;
+      bias[r] = a.bias && ch < a.n ? ld(a.bias + ch) : 0.0f;
+    }
+#pragma unroll
+    for (int j = 0; j < TM; ++j) {
+      const long row = m0 + wm + 32 * j + l31;
+      const float sx = row < a.m ? ld(a.sx + row) : 0.0f;
+      T* const yr = (T*)a.y + row * a.ldy;
+      float v[16];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) v[r] = i8_epilogue(acc[i][j][r], sx, sw[r], bias[r], a.act);
+      if (a.vec) {
+        // two groups of four channels per lane pair -> eight consecutive channels in one lane
+#pragma unroll
+        for (int q = 0; q < 4; q += 2) {
+          const int ch = n0 + wn + 32 * i + 8 * (q + half);
+          if constexpr (sizeof(T) == 2) {
+            unsigned lo[2] = {pack_bf16x2(v[4 * q], v[4 * q + 1]), pack_bf16x2(v[4 * q + 2], v[4 * q + 3])};
+            unsigned hi[2] = {pack_bf16x2(v[4 * q + 4], v[4 * q + 5]), pack_bf16x2(v[4 * q + 6], v[4 * q + 7])};
+            permlane32_swap(lo[0], hi[0]);
+            permlane32_swap(lo[1], hi[1]);
+            if (row < a.m && ch < a.n) st((uint4*)(yr + ch), make_uint4(lo[0], lo[1], hi[0], hi[1]));
+          } else {
+            unsigned lo[4], hi[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              lo[e] = f32_bits(v[4 * q + e]);
+              hi[e] = f32_bits(v[4 * q + 4 + e]);
+              permlane32_swap(lo[e], hi[e]);
+            }
+            if (row < a.m && ch < a.n) {
+              st((uint4*)(yr + ch), make_uint4(lo[0], lo[1], lo[2], lo[3]));
+              st((uint4*)(yr + ch + 4), make_uint4(hi[0], hi[1], hi[2], hi[3]));
+            }
+          }
+        }
+      } else if (row < a.m) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int ch = n0 + wn + 32 * i + (r & 3) + 8 * (r >> 2) + 4 * half;
+          if (ch < a.n) i8_store(yr + ch, v[r]);
+        }
+      }
+    }
+  }
+}
+
+// Joins the slices of a split sum (integers: any order gives the same) and finishes the outputs.
 template <typename T>
-__global__ __launch_bounds__(256) void inner_product_i8_kernel(const I8Args a) {
+__global__ __launch_bounds__(256) void i8_join_kernel(const I8Args a) {
   const long total = a.m * a.n;
   for (long o = (long)blockIdx.x * kI8Threads + threadIdx.x; o < total; o += (long)gridDim.x * kI8Threads) {
     const long i = o / a.n;
     const int j = (int)(o - i * a.n);
-    const signed char* xr = a.x + i * a.ldx;
-    const signed char* wr = a.w + j * a.ldw;
-    int acc = 0;
-    for (int l = 0; l < a.k; ++l) acc += (int)ld(xr + l) * (int)ld(wr + l);
-    i8_store((T*)a.y + i * a.ldy + j, i8_epilogue(acc, ld(a.sx + i), ld(a.sw + j), a.bias ? ld(a.bias + j) : 0.0f, a.act));
+    int sum = 0;
+    for (int s = 0; s < a.ksplit; ++s) sum += ld(a.part + s * total + o);
+    i8_store((T*)a.y + i * a.ldy + j, i8_epilogue(sum, ld(a.sx + i), ld(a.sw + j), a.bias ? ld(a.bias + j) : 0.0f, a.act));
   }
 }
 
 static inline unsigned i8_grid(long count, long per_block) {
   const long g = ceil_div(count, per_block);
   return (unsigned)(g > 1048576 ? 1048576 : g);   // grid-stride beyond this
+}
+
+constexpr int kTokMax = 32;     // rows up to which the token kernel is taken
+
+template <int BM, int BN, int WM, int WN, int NBUF, bool FAST, typename T>
+static int i8_launch_tile(I8Args& a, hipStream_t st) {
+  a.tiles_m = (int)ceil_div(a.m, BM);
+  a.tiles_n = (int)ceil_div(a.n, BN);
+  const int bufs = FAST ? (a.nstages < NBUF ? a.nstages : NBUF) : 2;
+  ECO_RAISE_DYNAMIC_LDS((i8_tile_kernel<BM, BN, WM, WN, NBUF, FAST, T>), "inner_product_i8");
+  hipLaunchKernelGGL((i8_tile_kernel<BM, BN, WM, WN, NBUF, FAST, T>), dim3((unsigned)(a.tiles_m * a.tiles_n * a.ksplit)),
+                     dim3(kI8Threads), (unsigned)(bufs * (BM + BN) * 64), st, a);
+  if (int rc = check_launch("eco_inner_product_i8_forward")) return rc;
+  if (a.ksplit > 1) {
+    hipLaunchKernelGGL((i8_join_kernel<T>), dim3(i8_grid(a.m * a.n, kI8Threads)), dim3(kI8Threads), 0, st, a);
+    return check_launch("eco_inner_product_i8_forward(join)");
+  }
+  return ECO_OK;
+}
+
+template <typename T>
+static int i8_launch(const eco_inner_product_i8_plan& p, I8Args& a, bool fast, hipStream_t st) {
+  if (a.m <= kTokMax) {
+    const dim3 grid((unsigned)ceil_div(a.n, 16)), block(kTokWaves * kWave);
+    if (a.m <= 16) {
+      if (fast) hipLaunchKernelGGL((i8_token_kernel<1, true, T>), grid, block, 0, st, a);
+      else hipLaunchKernelGGL((i8_token_kernel<1, false, T>), grid, block, 0, st, a);
+    } else {
+      if (fast) hipLaunchKernelGGL((i8_token_kernel<2, true, T>), grid, block, 0, st, a);
+      else hipLaunchKernelGGL((i8_token_kernel<2, false, T>), grid, block, 0, st, a);
+    }
+    return check_launch("eco_inner_product_i8_forward(tokens)");
+  }
+  if (fast) {
+    if (p.bm == 256) return i8_launch_tile<256, 256, 128, 128, 4, true, T>(a, st);
+    if (p.bm == 128) return i8_launch_tile<128, 128, 64, 64, 3, true, T>(a, st);
+    return i8_launch_tile<64, 64, 32, 32, 3, true, T>(a, st);
+  }
+  if (p.bm >= 128) return i8_launch_tile<128, 128, 64, 64, 3, false, T>(a, st);
+  return i8_launch_tile<64, 64, 32, 32, 3, false, T>(a, st);
 }
 
 }  // namespace eco
@@ -146,7 +493,26 @@ extern "C" int eco_inner_product_i8_plan_create(int64_t m, int64_t n, int64_t k,
   memset(plan, 0, sizeof(*plan));
   plan->m = m; plan->n = (int32_t)n; plan->k = (int32_t)k; plan->dt = dt;
   plan->num_cu = num_cu ? num_cu : current_device_num_cu();
-  plan->bm = plan->bn = 1; plan->ksplit = 1;
+  if (m <= kTokMax) {
+    plan->bm = m <= 16 ? 16 : 32; plan->bn = 16; plan->ksplit = 1;
+    return ECO_OK;
+  }
+  const long cu = plan->num_cu;
+  const auto tiles = [&](long bm, long bn) { return ceil_div(m, bm) * ceil_div(n, bn); };
+  // the largest tile that still gives every compute unit one; the smallest where none does
+  plan->bm = plan->bn = tiles(256, 256) >= cu ? 256 : tiles(128, 128) >= cu ? 128 : 64;
+  plan->ksplit = 1;
+  const long t = tiles(plan->bm, plan->bn), stages = ceil_div(k, 64);
+  ECO_REQUIRE(t <= 2147483647l / 16, "inner_product_i8: too many tiles for one launch");
+  if (t < cu && stages >= 16) {     // too few tiles: cut long sums so that two workgroups a compute unit run, of eight stages at least
+    long ks = ceil_div(2 * cu, t);
+    if (ks > stages / 8) ks = stages / 8;
+    if (ks > 16) ks = 16;
+    if (ks > 1) {
+      plan->ksplit = (int32_t)ks;
+      plan->ws_bytes = ks * m * n * 4;
+    }
+  }
   return ECO_OK;
 }
 
@@ -171,9 +537,15 @@ extern "C" int eco_inner_product_i8_forward(const eco_inner_product_i8_plan* pla
               "inner_product_i8: a row stride is too large");
   ECO_REQUIRE(plan->ws_bytes == 0 || workspace, "inner_product_i8: this plan needs %ld bytes of workspace", (long)plan->ws_bytes);
   a.m = plan->m; a.n = plan->n; a.k = plan->k; a.act = act;
-  hipStream_t st = (hipStream_t)stream;
-  const dim3 grid(i8_grid(a.m * a.n, kI8Threads)), block(kI8Threads);
-  if (plan->dt == ECO_DT_F32) hipLaunchKernelGGL((inner_product_i8_kernel<float>), grid, block, 0, st, a);
-  else hipLaunchKernelGGL((inner_product_i8_kernel<unsigned short>), grid, block, 0, st, a);
-  return check_launch("eco_inner_product_i8_forward");
+  a.part = (int*)workspace;
+  ECO_REQUIRE(plan->ws_bytes == 0 || (uintptr_t)workspace % 4 == 0, "inner_product_i8: workspace is not aligned to 4 bytes");
+  const size_t es = plan->dt == ECO_DT_F32 ? 4 : 2;
+  a.vec = a.n % 8 == 0 && (uintptr_t)y % 16 == 0 && (a.ldy * es) % 16 == 0;
+  a.ksplit = plan->ksplit;
+  a.nstages = (int)ceil_div(a.k, 64);
+  // 16-byte chunks of either operand inside its rows and on 16-byte boundaries; a tile's rows within the descriptors' 2 GB
+  const bool fast = a.k % 16 == 0 && a.ldx % 16 == 0 && a.ldw % 16 == 0 && ((uintptr_t)x | (uintptr_t)w) % 16 == 0 &&
+                    256 * a.ldx + a.k < 0x7fffffffl && 256 * a.ldw + a.k < 0x7fffffffl;
+  return plan->dt == ECO_DT_F32 ? i8_launch<float>(*plan, a, fast, (hipStream_t)stream)
+                                : i8_launch<unsigned short>(*plan, a, fast, (hipStream_t)stream);
 }

@@ -254,6 +254,15 @@ __device__ __forceinline__ void wait_dma_all_but() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 #endif
 }
+// This wave's LDS reads are in registers and its LDS writes done (s_waitcnt lgkmcnt(0), nothing else: the builtin, which the
+// compiler's own counting sees, so that it does not wait again behind it).
+__device__ __forceinline__ void wait_lds_reads() {
+#ifndef ECO_EMU
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0xc07f);
+  asm volatile("" ::: "memory");
+#endif
+}
 __device__ __forceinline__ void wg_barrier_nodrain() {
 #ifdef ECO_EMU
   emu::syncthreads();

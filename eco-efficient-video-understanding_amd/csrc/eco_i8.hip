@@ -81,11 +81,13 @@ struct I8Args {
 };
 
 // (int -> fp32 rounds once; the products and the sum once each)
-__device__ __forceinline__ float i8_epilogue(int acc, float sx, float sw, float bias, int act) {
-  float v = (float)acc * sx * sw + bias;
-  if (act == ECO_ACT_RELU) v = v < 0.0f ? 0.0f : v;
-  else if (act == ECO_ACT_SILU) v = v / (1.0f + expf(-v));
+__device__ __forceinline__ float i8_activate(float v, int act) {
+  if (act == ECO_ACT_RELU) return v < 0.0f ? 0.0f : v;
+  if (act == ECO_ACT_SILU) return v / (1.0f + expf(-v));
   return v;
+}
+__device__ __forceinline__ float i8_epilogue(int acc, float sx, float sw, float bias, int act) {
+  return i8_activate((float)acc * sx * sw + bias, act);
 }
 __device__ __forceinline__ void i8_store(float* p, float v) { st(p, v); }
 __device__ __forceinline__ void i8_store(unsigned short* p, float v) { st(p, (unsigned short)f32_to_bf16_bits(v)); }
@@ -108,12 +110,6 @@ __device__ __forceinline__ uint4 i8_chunk(const signed char* row, int at, int k)
   }
   return q;
 }
-template <bool FAST>
-__device__ __forceinline__ uint4 i8_chunk_of(const signed char* row, int at, int k) {
-  if constexpr (FAST) return at < k ? ld((const uint4*)(row + at)) : make_uint4(0u, 0u, 0u, 0u);
-  else return i8_chunk(row, at, k);
-}
-
 // ---- few tokens (m <= 32): bound by the weights' bytes ----------------------------------------------------------------------
 // A workgroup takes 16 output channels; its eight waves share the sum in units of 128 bytes.  Weights go from memory straight into
 // the matrix instruction's registers (16 rows x 64 bytes each), the tokens' bytes come from the caches in the same order of k,
@@ -126,15 +122,11 @@ __global__ __launch_bounds__(512) void i8_token_kernel(const I8Args a) {
   const int lane = lane_id(), wave = uniform((int)(threadIdx.x >> 6));
   const int n0 = (int)blockIdx.x * 16;
   const int r16 = lane & 15, kc = (lane >> 4) * 16;
-  const bool w_ok = n0 + r16 < a.n;
-  const signed char* wrow = a.w + (long)(w_ok ? n0 + r16 : 0) * a.ldw;
+  // (channels and tokens behind the last: the last one's bytes, their outputs are not stored)
+  const signed char* wrow = a.w + (long)(n0 + r16 < a.n ? n0 + r16 : a.n - 1) * a.ldw;
   const signed char* xrow[MT];
-  bool x_ok[MT];
 #pragma unroll
-  for (int t = 0; t < MT; ++t) {
-    x_ok[t] = t * 16 + r16 < a.m;
-    xrow[t] = a.x + (long)(x_ok[t] ? t * 16 + r16 : 0) * a.ldx;
-  }
+  for (int t = 0; t < MT; ++t) xrow[t] = a.x + (t * 16 + r16 < a.m ? t * 16 + r16 : a.m - 1) * a.ldx;
   i32x4 acc[MT];
 #pragma unroll
   for (int t = 0; t < MT; ++t) acc[t] = i32x4{0, 0, 0, 0};
@@ -145,11 +137,26 @@ __global__ __launch_bounds__(512) void i8_token_kernel(const I8Args a) {
     for (int f = 0; f < kTokFlight; ++f)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int at = (u0 + f * kTokWaves) * kTokUnit + h * 64 + kc;     // (past the end: zeros)
-        wq[f][h] = w_ok ? i8_chunk_of<FAST>(wrow, at, a.k) : make_uint4(0u, 0u, 0u, 0u);
+        const int at = (u0 + f * kTokWaves) * kTokUnit + h * 64 + kc;
+        if constexpr (FAST) {
+          // every load is issued: behind the end the row's last chunk again, with the weights zeroed
+          const int from = at < a.k ? at : a.k - 16;
+          wq[f][h] = ld((const uint4*)(wrow + from));
 #pragma unroll
-        for (int t = 0; t < MT; ++t) xq[f][h][t] = x_ok[t] ? i8_chunk_of<FAST>(xrow[t], at, a.k) : make_uint4(0u, 0u, 0u, 0u);
+          for (int t = 0; t < MT; ++t) xq[f][h][t] = ld((const uint4*)(xrow[t] + from));
+        } else {
+          wq[f][h] = i8_chunk(wrow, at, a.k);
+#pragma unroll
+          for (int t = 0; t < MT; ++t) xq[f][h][t] = i8_chunk(xrow[t], at, a.k);
+        }
       }
+    if constexpr (FAST) {
+#pragma unroll
+      for (int f = 0; f < kTokFlight; ++f)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          if ((u0 + f * kTokWaves) * kTokUnit + h * 64 + kc >= a.k) wq[f][h] = make_uint4(0u, 0u, 0u, 0u);
+    }
 #pragma unroll
     for (int f = 0; f < kTokFlight; ++f)
 #pragma unroll
@@ -187,6 +194,7 @@ __global__ __launch_bounds__(256, (BM * BN > 128 * 128) ? 1 : 2) void i8_tile_ke
   constexpr int TM = WM / 32, TN = WN / 32;              // 32x32 products of a wave
   constexpr int WAVES_N = BN / WN;
   static_assert((BM / WM) * (BN / WN) == 4, "four waves");
+  constexpr bool BIG = BM * BN > 128 * 128;              // (taken with whole sums and 16-byte stores only)
   constexpr int STAGE = (BM + BN) * 4;                   // 16-byte vectors of a stage: BN rows of w, then BM rows of x
   constexpr int PW = BN / 16 / 4, PX = BM / 16 / 4;      // DMA pieces (16 rows x 64 bytes) of a wave per stage
   ECO_DYNAMIC_LDS(lds_f);
@@ -217,18 +225,11 @@ __global__ __launch_bounds__(256, (BM * BN > 128 * 128) ? 1 : 2) void i8_tile_ke
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0;
 
   uint4 wf[2][TN], xf[2][TM];
-  auto read_frags = [&](int slot, const uint4* buf, int ks) {
+  // fragment r of k-step ks (r < TN: w's, else x's)
+  auto read_frag = [&](int slot, const uint4* buf, int ks, int r) {
     const int c = (2 * ks + half) ^ ((l31 >> 1) & 3);
-#pragma unroll
-    for (int i = 0; i < TN; ++i) wf[slot][i] = buf[(wn + 32 * i + l31) * 4 + c];
-#pragma unroll
-    for (int j = 0; j < TM; ++j) xf[slot][j] = buf[(BN + wm + 32 * j + l31) * 4 + c];
-  };
-  auto multiply = [&](int slot) {
-#pragma unroll
-    for (int i = 0; i < TN; ++i)
-#pragma unroll
-      for (int j = 0; j < TM; ++j) acc[i][j] = mfma_32x32x32_i8(wf[slot][i], xf[slot][j], acc[i][j]);
+    if (r < TN) wf[slot][r] = buf[(wn + 32 * r + l31) * 4 + c];
+    else xf[slot][r - TN] = buf[(BN + wm + 32 * (r - TN) + l31) * 4 + c];
   };
 
   if constexpr (FAST) {
@@ -243,88 +244,123 @@ __global__ __launch_bounds__(256, (BM * BN > 128 * 128) ? 1 : 2) void i8_tile_ke
     const int prow = lane >> 2, pchunk = (lane & 3) ^ ((prow >> 1) & 3);
     const unsigned vw = (unsigned)((long)prow * a.ldw + pchunk * 16), vx = (unsigned)((long)prow * a.ldx + pchunk * 16);
     const unsigned ldw16 = (unsigned)(16 * a.ldw), ldx16 = (unsigned)(16 * a.ldx);
-    auto issue = [&](int s) {           // stage s of this slice -> buffer s % NBUF
-      const int k0 = (s_begin + s) * 64;
-      const bool in_k = k0 + pchunk * 16 < a.k;            // (the last stage's chunks behind k: zeros)
-      const unsigned ow = in_k ? vw : kBufOob, ox = in_k ? vx : kBufOob;
+    // piece p (0 .. PW + PX - 1: w's, then x's) of stage s of this slice -> buffer s % NBUF
+    auto issue_piece = [&](int s, int p, unsigned ow, unsigned ox) {
+      const unsigned k0 = (unsigned)((s_begin + s) * 64);
       uint4* const buf = lds + (s % NBUF) * STAGE;
+      if (p < PW) glds16_buf(rw, ow, k0 + (unsigned)(p * 4 + wave) * ldw16, buf + (p * 4 + wave) * 64);
+      else glds16_buf(rx, ox, k0 + (unsigned)((p - PW) * 4 + wave) * ldx16, buf + BN * 4 + ((p - PW) * 4 + wave) * 64);
+    };
+    auto in_k = [&](int s) { return (s_begin + s) * 64 + pchunk * 16 < a.k; };   // (the last stage's chunks behind k: zeros)
+    auto issue = [&](int s) {
+      const unsigned ow = in_k(s) ? vw : kBufOob, ox = in_k(s) ? vx : kBufOob;
 #pragma unroll
-      for (int p = 0; p < PW; ++p) {
-        const int piece = p * 4 + wave;
-        glds16_buf(rw, ow, (unsigned)k0 + (unsigned)piece * ldw16, buf + piece * 64);
-      }
-#pragma unroll
-      for (int p = 0; p < PX; ++p) {
-        const int piece = p * 4 + wave;
-        glds16_buf(rx, ox, (unsigned)k0 + (unsigned)piece * ldx16, buf + BN * 4 + piece * 64);
-      }
+      for (int p = 0; p < PW + PX; ++p) issue_piece(s, p, ow, ox);
     };
     auto wait_stage = [&](int newer) {  // this wave's pieces of all but the newest `newer` stages have landed
       if (newer >= 2 && NBUF > 3) wait_dma_all_but<2 * (PW + PX)>();
       else if (newer >= 1) wait_dma_all_but<PW + PX>();
       else wait_dma_all_but<0>();
     };
+    // One half stage: the products of fragment set `slot`; between those of its first half the other set's fragments are read
+    // (k-step `ks` of buffer `buf`), between the rest, where `more`, the DMA pieces of stage s + NBUF are issued: the
+    // matrix unit works on meanwhile, and a fragment has half of the products' time to arrive.
+    auto half_stage = [&](auto slot_c, const uint4* buf, int ks, auto more_c, int s) {
+      constexpr int slot = decltype(slot_c)::value;
+      constexpr bool more = decltype(more_c)::value;
+      constexpr int NP = TN * TM, NR = TN + TM;
+      unsigned ow = 0, ox = 0;
+      if constexpr (more) { ow = in_k(s + NBUF) ? vw : kBufOob; ox = in_k(s + NBUF) ? vx : kBufOob; }
+      static_for<NP>([&](auto qc) {
+        constexpr int q = decltype(qc)::value, i = q / TM, j = q % TM;
+        acc[i][j] = mfma_32x32x32_i8(wf[slot][i], xf[slot][j], acc[i][j]);
+        sched_fence();
+        if (buf) {
+          constexpr int r0 = 2 * q * NR / NP < NR ? 2 * q * NR / NP : NR, r1 = 2 * (q + 1) * NR / NP < NR ? 2 * (q + 1) * NR / NP : NR;
+#pragma unroll
+          for (int r = r0; r < r1; ++r) read_frag(slot ^ 1, buf, ks, r);
+        }
+        if constexpr (more) {
+          constexpr int h = NP / 2, p0 = q < h ? 0 : (q - h) * (PW + PX) / (NP - h), p1 = q < h ? 0 : (q + 1 - h) * (PW + PX) / (NP - h);
+#pragma unroll
+          for (int p = p0; p < p1; ++p) issue_piece(s + NBUF, p, ow, ox);
+        }
+        sched_fence();
+      });
+    };
     for (int s = 0; s < NBUF - 1 && s < ns; ++s) issue(s);
-    {
-      const int newer = (ns < NBUF - 1 ? ns : NBUF - 1) - 1;
-      wait_stage(newer);
-    }
+    wait_stage((ns < NBUF - 1 ? ns : NBUF - 1) - 1);
     wg_barrier_nodrain();
-    // one more stage ahead than the buffers behind the barrier above: buffer NBUF - 1 is still empty
+    // one more stage ahead than in the loop: buffer NBUF - 1 is still empty
     if (NBUF - 1 < ns) issue(NBUF - 1);
-    read_frags(0, lds, 0);
-    for (int s = 0; s < ns; ++s) {
-      read_frags(1, lds + (s % NBUF) * STAGE, 1);
-      multiply(0);
-      if (s + 1 < ns) {
-        // stages s+1 .. min(s+NBUF-1, ns-1) are in flight: s+1 must have landed
-        const int newer = (ns - 1 < s + NBUF - 1 ? ns - 1 : s + NBUF - 1) - (s + 1);
-        wait_stage(newer);
-#ifndef ECO_EMU
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // this wave's fragments of stage s are in registers
-#endif
-        wg_barrier_nodrain();
-        if (s + NBUF < ns) issue(s + NBUF);                  // into the buffer that stage s leaves
-        read_frags(0, lds + ((s + 1) % NBUF) * STAGE, 0);
-      }
-      multiply(1);
+#pragma unroll
+    for (int r = 0; r < TN + TM; ++r) read_frag(0, lds, 0, r);
+    constexpr std::integral_constant<int, 0> c0{};
+    constexpr std::integral_constant<int, 1> c1{};
+    constexpr std::false_type no{};
+    constexpr std::true_type yes{};
+    int s = 0;
+    for (; s + NBUF < ns; ++s) {
+      half_stage(c0, lds + (s % NBUF) * STAGE, 1, no, 0);
+      wait_lds_reads();                                  // this wave's fragments of stage s are in registers
+      wait_dma_all_but<(NBUF - 2) * (PW + PX)>();        // stages s+1 .. s+NBUF-1 are in flight: s+1 has landed
+      wg_barrier_nodrain();
+      half_stage(c1, lds + ((s + 1) % NBUF) * STAGE, 0, yes, s);   // stage s+NBUF into the buffer that stage s leaves
     }
+    for (; s + 1 < ns; ++s) {
+      half_stage(c0, lds + (s % NBUF) * STAGE, 1, no, 0);
+      wait_lds_reads();
+      wait_stage(ns - 1 - (s + 1));
+      wg_barrier_nodrain();
+      half_stage(c1, lds + ((s + 1) % NBUF) * STAGE, 0, no, 0);
+    }
+    half_stage(c0, lds + (s % NBUF) * STAGE, 1, no, 0);
+    half_stage(c1, nullptr, 0, no, 0);
   } else {
     constexpr int CH = STAGE / 256;       // chunks of a thread per stage
-    uint4 q[CH];
-    auto fetch = [&](int s) {
+    constexpr int AHEAD = BM * BN > 64 * 64 ? 2 : 4;   // stages in registers
+    uint4 q[AHEAD][CH];
+    auto fetch = [&](int s, uint4 (&to)[CH]) {
       const int k0 = (s_begin + s) * 64;
 #pragma unroll
       for (int p = 0; p < CH; ++p) {
         const int id4 = p * 256 + tid, row = id4 >> 2, at = k0 + (id4 & 3) * 16;
-        q[p] = make_uint4(0u, 0u, 0u, 0u);
-        if (row < BN) { if (n0 + row < a.n) q[p] = i8_chunk(a.w + (long)(n0 + row) * a.ldw, at, a.k); }
-        else if (m0 + row - BN < a.m) q[p] = i8_chunk(a.x + (m0 + row - BN) * a.ldx, at, a.k);
+        to[p] = make_uint4(0u, 0u, 0u, 0u);
+        if (row < BN) { if (n0 + row < a.n) to[p] = i8_chunk(a.w + (long)(n0 + row) * a.ldw, at, a.k); }
+        else if (m0 + row - BN < a.m) to[p] = i8_chunk(a.x + (m0 + row - BN) * a.ldx, at, a.k);
       }
     };
-    auto put = [&](int s) {
+    static_for<AHEAD>([&](auto d) { if (decltype(d)::value < ns) fetch(decltype(d)::value, q[decltype(d)::value]); });
+    for (int s0 = 0; s0 < ns; s0 += AHEAD)
+      static_for<AHEAD>([&](auto d) {
+        constexpr int v = decltype(d)::value;
+        const int s = s0 + v;
+        if (s < ns) {
+          uint4* const buf = lds + (s & 1) * STAGE;
 #pragma unroll
-      for (int p = 0; p < CH; ++p) {
-        const int id4 = p * 256 + tid, row = id4 >> 2;
-        lds[(s & 1) * STAGE + row * 4 + ((id4 & 3) ^ ((row >> 1) & 3))] = q[p];
-      }
-    };
-    fetch(0);
-    put(0);
-    __syncthreads();
-    for (int s = 0; s < ns; ++s) {
-      if (s + 1 < ns) fetch(s + 1);
-      read_frags(0, lds + (s & 1) * STAGE, 0);
-      read_frags(1, lds + (s & 1) * STAGE, 1);
-      multiply(0);
-      multiply(1);
-      if (s + 1 < ns) put(s + 1);
-      __syncthreads();
-    }
+          for (int p = 0; p < CH; ++p) {
+            const int id4 = p * 256 + tid, row = id4 >> 2;
+            buf[row * 4 + ((id4 & 3) ^ ((row >> 1) & 3))] = q[v][p];
+          }
+          if (s + AHEAD < ns) fetch(s + AHEAD, q[v]);
+          // (one barrier a stage: a wave may write buffer s+1 -- last read in stage s-1 -- while others still read buffer s)
+          wait_lds_reads();
+          wg_barrier_nodrain();
+#pragma unroll
+          for (int ks = 0; ks < 2; ++ks) {
+#pragma unroll
+            for (int r = 0; r < TN + TM; ++r) read_frag(0, buf, ks, r);
+#pragma unroll
+            for (int i = 0; i < TN; ++i)
+#pragma unroll
+              for (int j = 0; j < TM; ++j) acc[i][j] = mfma_32x32x32_i8(wf[0][i], xf[0][j], acc[i][j]);
+          }
+        }
+      });
   }
 
   // ---- epilogue: a lane holds row m0 + wm + 32 j + l31 and channels 8 q + 4 half + {0..3}, q = 0..3, of each 32-channel block
-  if (a.ksplit > 1) {
+  if (!BIG && a.ksplit > 1) {
 #pragma unroll
     for (int j = 0; j < TM; ++j) {
       const long row = m0 + wm + 32 * j + l31;
@@ -341,24 +377,34 @@ __global__ __launch_bounds__(256, (BM * BN > 128 * 128) ? 1 : 2) void i8_tile_ke
     }
     return;
   }
+  float sx[TM];
+#pragma unroll
+  for (int j = 0; j < TM; ++j) {
+    const long row = m0 + wm + 32 * j + l31;
+    sx[j] = ld(a.sx + (row < a.m ? row : a.m - 1));      // (rows and channels behind the last: any value, never stored)
+  }
 #pragma unroll
   for (int i = 0; i < TN; ++i) {
     float sw[16], bias[16];
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      const int ch = n0 + wn + 32 * i + (r & 3) + 8 * (r >> 2) + 4 * half;
-      sw[r] = ch < a.n ? ld(a.sw + ch) : 0.0f;
-      bias[r] = a.bias && ch < a.n ? ld(a.bias + ch) : 0.0f;
+      int ch = n0 + wn + 32 * i + (r & 3) + 8 * (r >> 2) + 4 * half;
+      ch = ch < a.n ? ch : a.n - 1;
+      sw[r] = ld(a.sw + ch);
+      bias[r] = a.bias ? ld(a.bias + ch) : 0.0f;
     }
 #pragma unroll
     for (int j = 0; j < TM; ++j) {
       const long row = m0 + wm + 32 * j + l31;
-      const float sx = row < a.m ? ld(a.sx + row) : 0.0f;
       T* const yr = (T*)a.y + row * a.ldy;
       float v[16];
 #pragma unroll
-      for (int r = 0; r < 16; ++r) v[r] = i8_epilogue(acc[i][j][r], sx, sw[r], bias[r], a.act);
-      if (a.vec) {
+      for (int r = 0; r < 16; ++r) v[r] = (float)acc[i][j][r] * sx[j] * sw[r] + bias[r];
+      if (a.act != ECO_ACT_NONE) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) v[r] = i8_activate(v[r], a.act);
+      }
+      if (BIG || a.vec) {
         // two groups of four channels per lane pair -> eight consecutive channels in one lane
 #pragma unroll
         for (int q = 0; q < 4; q += 2) {
@@ -444,8 +490,8 @@ static int i8_launch(const eco_inner_product_i8_plan& p, I8Args& a, bool fast, h
     return check_launch("eco_inner_product_i8_forward(tokens)");
   }
   if (fast) {
-    if (p.bm == 256) return i8_launch_tile<256, 256, 128, 128, 4, true, T>(a, st);
-    if (p.bm == 128) return i8_launch_tile<128, 128, 64, 64, 3, true, T>(a, st);
+    if (p.bm == 256 && a.vec) return i8_launch_tile<256, 256, 128, 128, 4, true, T>(a, st);
+    if (p.bm >= 128) return i8_launch_tile<128, 128, 64, 64, 3, true, T>(a, st);
     return i8_launch_tile<64, 64, 32, 32, 3, true, T>(a, st);
   }
   if (p.bm >= 128) return i8_launch_tile<128, 128, 64, 64, 3, false, T>(a, st);
@@ -497,14 +543,20 @@ extern "C" int eco_inner_product_i8_plan_create(int64_t m, int64_t n, int64_t k,
     plan->bm = m <= 16 ? 16 : 32; plan->bn = 16; plan->ksplit = 1;
     return ECO_OK;
   }
-  const long cu = plan->num_cu;
+  // The tile with the least time by a model in cycles of a compute unit: rounds of tiles x (stages x cost of a stage + cost of
+  // a tile's start and end).  A stage of 64 bytes costs a 256 x 256 tile its products (1024 cycles, the LDS three quarters
+  // busy), smaller tiles their LDS traffic (48 and 24 KB at 128 bytes a cycle); starts and ends hide behind the
+  // neighbours that the smaller tiles' LDS leaves room for.
+  const long cu = plan->num_cu, stages = ceil_div(k, 64);
   const auto tiles = [&](long bm, long bn) { return ceil_div(m, bm) * ceil_div(n, bn); };
-  // the largest tile that still gives every compute unit one; the smallest where none does
-  plan->bm = plan->bn = tiles(256, 256) >= cu ? 256 : tiles(128, 128) >= cu ? 128 : 64;
+  const auto cost = [&](long b, long stage, long ends) { return ceil_div(tiles(b, b), cu) * (stages * stage + ends); };
+  const long c256 = cost(256, 1300, 8000), c128 = cost(128, 420, 2000), c64 = cost(64, 210, 900);
+  const bool big = n % 8 == 0 && c256 <= c128 && c256 <= c64;      // (its stores are 16 bytes wide)
+  plan->bm = plan->bn = big ? 256 : c128 <= c64 ? 128 : 64;
   plan->ksplit = 1;
-  const long t = tiles(plan->bm, plan->bn), stages = ceil_div(k, 64);
+  const long t = tiles(plan->bm, plan->bn);
   ECO_REQUIRE(t <= 2147483647l / 16, "inner_product_i8: too many tiles for one launch");
-  if (t < cu && stages >= 16) {     // too few tiles: cut long sums so that two workgroups a compute unit run, of eight stages at least
+  if (!big && t < cu && stages >= 16) {     // too few tiles: cut long sums so that two workgroups a compute unit run, of eight stages at least
     long ks = ceil_div(2 * cu, t);
     if (ks > stages / 8) ks = stages / 8;
     if (ks > 16) ks = 16;

@@ -163,10 +163,12 @@ __device__ __forceinline__ uint4 gld16_buf(const BufRd& r, unsigned voff) {
 struct BufRsrc { const char* base; unsigned bytes; };
 __device__ __forceinline__ BufRsrc make_buf_rsrc(const void* p, unsigned bytes) { return BufRsrc{(const char*)p, bytes}; }
 __device__ __forceinline__ void glds16_buf(const BufRsrc& r, unsigned voff, unsigned soff, uint4* lds_wave_base) {
-  uint4 q = {0u, 0u, 0u, 0u};
-  const unsigned long long off = (unsigned long long)voff + soff;
-  if (off + 16 <= r.bytes && emu::check_access(r.base + off, 16, false)) memcpy(&q, r.base + off, 16);
-  lds_wave_base[emu::tls_cur->lane] = q;
+  unsigned q[4] = {0u, 0u, 0u, 0u};   // (the range check is per dword, as gld16_buf's)
+  for (int i = 0; i < 4; ++i) {
+    const unsigned long long off = (unsigned long long)voff + soff + 4 * i;
+    if (off + 4 <= r.bytes && emu::check_access(r.base + off, 4, false)) memcpy(&q[i], r.base + off, 4);
+  }
+  lds_wave_base[emu::tls_cur->lane] = make_uint4(q[0], q[1], q[2], q[3]);
 }
 #else
 typedef int BufRsrc __attribute__((ext_vector_type(4)));
@@ -324,6 +326,16 @@ __device__ __forceinline__ float shfl_xor(float v, int mask) {
   return emu::wave_xchg_f32(v, emu::tls_cur->lane ^ mask);
 #else
   return __shfl_xor(v, mask, 64);
+#endif
+}
+
+// v / (1 + exp(-v)) on the hardware's 2^x and reciprocal (one unit in the last place each): off by at most (7 + |v|) * 2^-24
+// relative; 0 below v = -89, where the value is under 2^-120.
+__device__ __forceinline__ float silu(float v) {
+#ifdef ECO_EMU
+  return v * (1.0f / (1.0f + exp2f(v * -1.44269504f)));
+#else
+  return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(v * -1.44269504f));
 #endif
 }
 

@@ -33,7 +33,7 @@ __device__ __forceinline__ void gn_store(unsigned short* p, float v) { st(p, (un
 
 __device__ __forceinline__ float gn_act(float v, int act) {
   if (act == ECO_ACT_RELU) return v < 0.0f ? 0.0f : v;      // (a NaN stays)
-  if (act == ECO_ACT_SILU) return v / (1.0f + expf(-v));
+  if (act == ECO_ACT_SILU) return silu(v);
   return v;
 }
 

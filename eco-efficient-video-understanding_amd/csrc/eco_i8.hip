@@ -83,7 +83,7 @@ struct I8Args {
 // (int -> fp32 rounds once; the products and the sum once each)
 __device__ __forceinline__ float i8_activate(float v, int act) {
   if (act == ECO_ACT_RELU) return v < 0.0f ? 0.0f : v;
-  if (act == ECO_ACT_SILU) return v / (1.0f + expf(-v));
+  if (act == ECO_ACT_SILU) return silu(v);
   return v;
 }
 __device__ __forceinline__ float i8_epilogue(int acc, float sx, float sw, float bias, int act) {
@@ -182,261 +182,338 @@ __global__ __launch_bounds__(512) void i8_token_kernel(const I8Args a) {
 }
 
 // ---- tiles on the matrix cores -------------------------------------------------------------------------------------------------
-// A workgroup of four waves takes BN output channels x BM rows, each wave WN x WM of them as 32x32 products
-// (D's rows are channels, so that a lane ends up with consecutive channels of one row of y).  Both operands pass through LDS in
-// stages of 64 bytes of k, rows 64 bytes apart, the four 16-byte chunks of row r stored in the order c ^ ((r >> 1) & 3): eight
-// lanes that read a fragment then touch all 32 banks once.
-//   FAST  (rows on 16-byte boundaries, k a multiple of 16): LDS-DMA into NBUF buffers, NBUF - 1 stages ahead; a buffer is refilled
-//         behind the barrier in the middle of its own stage, when every wave has its last fragments in registers
-//   else  any alignment: through registers, one stage ahead, two buffers
-template <int BM, int BN, int WM, int WN, int NBUF, bool FAST, typename T>
-__global__ __launch_bounds__(256, (BM * BN > 128 * 128) ? 1 : 2) void i8_tile_kernel(const I8Args a) {
-  constexpr int TM = WM / 32, TN = WN / 32;              // 32x32 products of a wave
-  constexpr int WAVES_N = BN / WN;
-  static_assert((BM / WM) * (BN / WN) == 4, "four waves");
-  constexpr bool BIG = BM * BN > 128 * 128;              // (taken with whole sums and 16-byte stores only)
-  constexpr int STAGE = (BM + BN) * 4;                   // 16-byte vectors of a stage: BN rows of w, then BM rows of x
-  constexpr int PW = BN / 16 / 4, PX = BM / 16 / 4;      // DMA pieces (16 rows x 64 bytes) of a wave per stage
+// A workgroup of four waves takes B output channels x B rows, each wave W x W of them (W = B / 2) as 32x32 products (D's rows are
+// channels, so that a lane ends up with consecutive channels of one row of y).  Both operands pass through LDS in stages of
+// 64 bytes of k, rows 64 bytes apart, the four 16-byte chunks of row r stored in the order c ^ ((r >> 2) & 3): sixteen lanes
+// that read a fragment then touch all 64 banks once.
+//   FAST  (rows on 16-byte boundaries, k a multiple of 16): persistent workgroups walk their tiles' stages as ONE stream through
+//         NBUF buffers filled by LDS-DMA, up to NBUF stages ahead -- across the ends of tiles, so that a tile's stores
+//         run under the next one's loads.  (The 256 tile's sums fill the accumulator file, fragments held across its end
+//         spill: one tile a workgroup.)  A buffer is refilled behind the barrier in the middle of its own stage, when every
+//         wave has its last fragments in registers.  A tile's scales and bias come the same way, into one of three slots.
+//   else  any alignment: one tile a workgroup, operands through registers
+template <int B, int NBUF, bool FAST, typename T>
+__global__ __launch_bounds__(256, B > 128 ? 1 : 3) void i8_tile_kernel(const I8Args a) {
+  constexpr int W = B / 2, TW = W / 32;                  // TW x TW products of 32x32 a wave
+  constexpr bool BIG = B > 128;                          // (taken with whole sums and 16-byte stores only)
+  constexpr int STAGE = 2 * B * 4;                       // 16-byte vectors of a stage: B rows of w, then B rows of x
+  constexpr int NR = 2 * TW, NP = TW * TW;               // fragments and products of a k-step
+  constexpr int PW = B / 64;                             // DMA pieces (16 rows x 64 bytes) of a wave per stage and operand
+  constexpr int SLOT = 3 * B;                            // floats of a tile's parameters: sw, bias, sx
   ECO_DYNAMIC_LDS(lds_f);
   uint4* const lds = (uint4*)lds_f;
+  float* const params = lds_f + NBUF * STAGE * 4;
   const int tid = (int)threadIdx.x, lane = lane_id(), wave = uniform(tid >> 6);
   const int half = lane >> 5, l31 = lane & 31;
+  const int wn = (wave & 1) * W, wm = (wave >> 1) * W;
 
-  // XCD-contiguous tile numbers, then groups of eight row tiles by all channel tiles: the tiles that run side by side on an XCD
-  // share their operands through its L2
-  const int tiles = a.tiles_m * a.tiles_n;
-  const int id = xcd_remap((int)blockIdx.x, tiles * a.ksplit);
-  const int slice = id / tiles, tile = id - slice * tiles;
-  const int per = 8 * a.tiles_n, grp = tile / per, first = grp * 8;
-  const int gm = a.tiles_m - first < 8 ? a.tiles_m - first : 8;
-  const int in = tile - grp * per;
-  const long m0 = (long)(first + in % gm) * BM;
-  const int n0 = (in / gm) * BN;
-  const int s_begin = (int)((long)a.nstages * slice / a.ksplit), s_end = (int)((long)a.nstages * (slice + 1) / a.ksplit);
-  const int ns = s_end - s_begin;
-
-  const int wn = (wave % WAVES_N) * WN, wm = (wave / WAVES_N) * WM;
-  i32x16 acc[TN][TM];
-#pragma unroll
-  for (int i = 0; i < TN; ++i)
-#pragma unroll
-    for (int j = 0; j < TM; ++j)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0;
-
-  uint4 wf[2][TN], xf[2][TM];
-  // fragment r of k-step ks (r < TN: w's, else x's)
-  auto read_frag = [&](int slot, const uint4* buf, int ks, int r) {
-    const int c = (2 * ks + half) ^ ((l31 >> 1) & 3);
-    if (r < TN) wf[slot][r] = buf[(wn + 32 * r + l31) * 4 + c];
-    else xf[slot][r - TN] = buf[(BN + wm + 32 * (r - TN) + l31) * 4 + c];
+  // Tile numbers: XCD b % 8 owns a contiguous range, its workgroups take every gx-th of it; inside, groups of eight row tiles
+  // by all channel tiles: the tiles that run side by side on an XCD share their operands through its L2.
+  const int tiles = a.tiles_m * a.tiles_n, total = tiles * a.ksplit;
+  const int xcd = (int)blockIdx.x & 7, gx = ((int)gridDim.x - xcd + 7) >> 3;
+  const int xbase = xcd * (total >> 3) + (xcd < (total & 7) ? xcd : (total & 7));
+  const int xend = xbase + (total >> 3) + (xcd < (total & 7) ? 1 : 0);
+  struct Item {
+    long m0;
+    int n0, slice, s_begin, ns;
+  };
+  auto item_of = [&](int id) {
+    Item t;
+    t.slice = id / tiles;
+    const int tile = id - t.slice * tiles;
+    const int per = 8 * a.tiles_n, grp = tile / per, in = tile - grp * per;
+    const int gm = a.tiles_m - 8 * grp < 8 ? a.tiles_m - 8 * grp : 8;
+    const int q = in / gm;
+    t.m0 = (long)uniform(8 * grp + in - q * gm) * B;
+    t.n0 = uniform(q * B);
+    t.slice = uniform(t.slice);
+    t.s_begin = uniform(a.nstages * t.slice / a.ksplit);              // (at most 2048 stages, 16 slices)
+    // (two stages at least: a tile's parameters are asked for at most two tiles ahead; the stage behind k is zeros)
+    const int ns = uniform(a.nstages * (t.slice + 1) / a.ksplit) - t.s_begin;
+    t.ns = ns < 2 ? 2 : ns;
+    return t;
   };
 
+  i32x16 acc[TW][TW];
+  auto clear = [&]() {
+#pragma unroll
+    for (int i = 0; i < TW; ++i)
+#pragma unroll
+      for (int j = 0; j < TW; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[i][j][r] = 0;
+  };
+  uint4 wf[2][TW], xf[2][TW];
+  // fragment r of k-step ks (r < TW: w's, else x's)
+  const int fsw = (l31 >> 2) & 3, fw = (wn + l31) * 4, fx = (B + wm + l31) * 4;
+  const int fk[2] = {half ^ fsw, (2 + half) ^ fsw};
+  auto read_frag = [&](int slot, const uint4* buf, int ks, int r) {
+    if (r < TW) wf[slot][r] = buf[fw + fk[ks] + 128 * r];
+    else xf[slot][r - TW] = buf[fx + fk[ks] + 128 * (r - TW)];
+  };
+
+  // A lane holds row m0 + wm + 32 j + l31 and channels 8 q + 4 half + {0..3}, q = 0..3, of each 32-channel block.
+  auto finish = [&](const Item& t, const float* par) {
+    // (opaque per tile: as invariants of the tile loop their many addresses would be computed once and live in scratch memory)
+    int l31 = lane & 31, half = lane >> 5;
+    ECO_OPAQUE(l31);
+    ECO_OPAQUE(half);
+    if (!BIG && a.ksplit > 1) {
+#pragma unroll
+      for (int j = 0; j < TW; ++j) {
+        const long row = t.m0 + wm + 32 * j + l31;
+        if (row < a.m) {
+          int* const to = a.part + ((long)t.slice * a.m + row) * a.n;
+#pragma unroll
+          for (int i = 0; i < TW; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const int ch = t.n0 + wn + 32 * i + (r & 3) + 8 * (r >> 2) + 4 * half;
+              if (ch < a.n) st(to + ch, acc[i][j][r]);
+            }
+        }
+      }
+      return;
+    }
+    float sx[TW];
+#pragma unroll
+    for (int j = 0; j < TW; ++j) sx[j] = par[2 * B + wm + 32 * j + l31];
+#pragma unroll
+    for (int i = 0; i < TW; ++i) {
+      sched_fence();          // (one block's parameters in registers at a time)
+      float4 sw[4], bias[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        sw[q] = *(const float4*)(par + wn + 32 * i + 8 * q + 4 * half);
+        bias[q] = *(const float4*)(par + B + wn + 32 * i + 8 * q + 4 * half);
+      }
+#pragma unroll
+      for (int j = 0; j < TW; ++j) {
+        sched_fence();
+        const long row = t.m0 + wm + 32 * j + l31;
+        T* const yr = (T*)a.y + row * a.ldy;
+        float v[16];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const i32x16& c = acc[i][j];
+          v[4 * q] = (float)c[4 * q] * sx[j] * sw[q].x + bias[q].x;
+          v[4 * q + 1] = (float)c[4 * q + 1] * sx[j] * sw[q].y + bias[q].y;
+          v[4 * q + 2] = (float)c[4 * q + 2] * sx[j] * sw[q].z + bias[q].z;
+          v[4 * q + 3] = (float)c[4 * q + 3] * sx[j] * sw[q].w + bias[q].w;
+        }
+        if (a.act == ECO_ACT_RELU) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) v[r] = i8_activate(v[r], ECO_ACT_RELU);
+        } else if (a.act == ECO_ACT_SILU) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) v[r] = i8_activate(v[r], ECO_ACT_SILU);
+        }
+        if (BIG || a.vec) {
+          // two groups of four channels per lane pair -> eight consecutive channels in one lane
+#pragma unroll
+          for (int q = 0; q < 4; q += 2) {
+            const int ch = t.n0 + wn + 32 * i + 8 * (q + half);
+            if constexpr (sizeof(T) == 2) {
+              unsigned lo[2] = {pack_bf16x2(v[4 * q], v[4 * q + 1]), pack_bf16x2(v[4 * q + 2], v[4 * q + 3])};
+              unsigned hi[2] = {pack_bf16x2(v[4 * q + 4], v[4 * q + 5]), pack_bf16x2(v[4 * q + 6], v[4 * q + 7])};
+              permlane32_swap(lo[0], hi[0]);
+              permlane32_swap(lo[1], hi[1]);
+              if (row < a.m && ch < a.n) st((uint4*)(yr + ch), make_uint4(lo[0], lo[1], hi[0], hi[1]));
+            } else {
+              unsigned lo[4], hi[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                lo[e] = f32_bits(v[4 * q + e]);
+                hi[e] = f32_bits(v[4 * q + 4 + e]);
+                permlane32_swap(lo[e], hi[e]);
+              }
+              if (row < a.m && ch < a.n) {
+                st((uint4*)(yr + ch), make_uint4(lo[0], lo[1], lo[2], lo[3]));
+                st((uint4*)(yr + ch + 4), make_uint4(hi[0], hi[1], hi[2], hi[3]));
+              }
+            }
+          }
+        } else if (row < a.m) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int ch = t.n0 + wn + 32 * i + (r & 3) + 8 * (r >> 2) + 4 * half;
+            if (ch < a.n) i8_store(yr + ch, v[r]);
+          }
+        }
+      }
+    }
+  };
+
+  clear();
+  int id = xbase + ((int)blockIdx.x >> 3);
+  Item cur = item_of(id);
+
   if constexpr (FAST) {
-    // descriptors from the tile's first row to the operand's end: rows behind the last one read zeros
-    const long wext = (long)(a.n - n0 - 1) * a.ldw + a.k, xext = (a.m - m0 - 1) * a.ldx + a.k;
-    const BufRsrc rw = make_buf_rsrc(a.w + (long)n0 * a.ldw, (unsigned)(wext < 0x7fffffffl ? wext : 0x7fffffffl));
-    const BufRsrc rx = make_buf_rsrc(a.x + m0 * a.ldx, (unsigned)(xext < 0x7fffffffl ? xext : 0x7fffffffl));
-#ifndef ECO_EMU
-    // (descriptor words written by readfirstlane: five wait states before a memory instruction inside asm may read them)
-    asm volatile("s_nop 4" ::"s"(rw), "s"(rx));
-#endif
-    const int prow = lane >> 2, pchunk = (lane & 3) ^ ((prow >> 1) & 3);
+    const int prow = lane >> 2, pchunk = (lane & 3) ^ (prow >> 2);
     const unsigned vw = (unsigned)((long)prow * a.ldw + pchunk * 16), vx = (unsigned)((long)prow * a.ldx + pchunk * 16);
     const unsigned ldw16 = (unsigned)(16 * a.ldw), ldx16 = (unsigned)(16 * a.ldx);
-    // piece p (0 .. PW + PX - 1: w's, then x's) of stage s of this slice -> buffer s % NBUF
-    auto issue_piece = [&](int s, int p, unsigned ow, unsigned ox) {
-      const unsigned k0 = (unsigned)((s_begin + s) * 64);
-      uint4* const buf = lds + (s % NBUF) * STAGE;
+    // ---- the asking side of the stream: item, stage in it, its operands' descriptors (from the tile's first row to the
+    // operand's end: rows behind the last one read zeros) ----
+    Item ask = cur;
+    int ask_id = id, ask_s = 0, ask_tile = 0, asked = 0;
+    bool ask_more = true;
+    BufRsrc rw, rx;
+    auto describe = [&]() {
+      const long wext = (long)(a.n - ask.n0 - 1) * a.ldw + a.k, xext = (a.m - ask.m0 - 1) * a.ldx + a.k;
+      rw = make_buf_rsrc(a.w + (long)ask.n0 * a.ldw, (unsigned)(wext < 0x7fffffffl ? wext : 0x7fffffffl));
+      rx = make_buf_rsrc(a.x + ask.m0 * a.ldx, (unsigned)(xext < 0x7fffffffl ? xext : 0x7fffffffl));
+      // the tile's parameters: one piece by each of three waves (sw, bias -- none: zeros --, sx); lanes behind B / 4 stay out
+      if (wave < 3) {
+        const float* from = wave == 0 ? a.sw + ask.n0 : wave == 1 ? (a.bias ? a.bias + ask.n0 : a.sw) : a.sx + ask.m0;
+        const long left = wave == 2 ? a.m - ask.m0 : wave == 1 && !a.bias ? 0 : (long)(a.n - ask.n0);
+        const BufRsrc rp = make_buf_rsrc(from, (unsigned)(4 * (left < B ? left : B)));
+#ifndef ECO_EMU
+        asm volatile("s_nop 4" ::"s"(rp));
+#endif
+        if (lane < B / 4) glds16_buf(rp, (unsigned)lane * 16u, 0u, (uint4*)(params + (ask_tile % 3) * SLOT + wave * B));
+      }
+#ifndef ECO_EMU
+      // (descriptor words written by readfirstlane: five wait states before a memory instruction inside asm may read them)
+      asm volatile("s_nop 4" ::"s"(rw), "s"(rx));
+#endif
+    };
+    // piece p (0 .. 2 PW - 1: w's, then x's) of the stage that is asked for next
+    auto ask_piece = [&](int p, unsigned k0, unsigned ow, unsigned ox) {
+      uint4* const buf = lds + (asked % NBUF) * STAGE;
       if (p < PW) glds16_buf(rw, ow, k0 + (unsigned)(p * 4 + wave) * ldw16, buf + (p * 4 + wave) * 64);
-      else glds16_buf(rx, ox, k0 + (unsigned)((p - PW) * 4 + wave) * ldx16, buf + BN * 4 + ((p - PW) * 4 + wave) * 64);
+      else glds16_buf(rx, ox, k0 + (unsigned)((p - PW) * 4 + wave) * ldx16, buf + B * 4 + ((p - PW) * 4 + wave) * 64);
     };
-    auto in_k = [&](int s) { return (s_begin + s) * 64 + pchunk * 16 < a.k; };   // (the last stage's chunks behind k: zeros)
-    auto issue = [&](int s) {
-      const unsigned ow = in_k(s) ? vw : kBufOob, ox = in_k(s) ? vx : kBufOob;
+    auto ask_k0 = [&]() { return (unsigned)((ask.s_begin + ask_s) * 64); };
+    // (chunks behind k, and the stages asked for behind the stream's end: zeros, nothing is read)
+    auto ask_in_k = [&]() { return ask_more && (int)ask_k0() + pchunk * 16 < a.k; };
+    auto ask_next = [&]() {             // one stage further
+      ++asked;
+      if (++ask_s == ask.ns && ask_more) {
+        ask_s = 0;
+        ask_id += gx;
+        ++ask_tile;
+        ask_more = !BIG && ask_id < xend;
+        if (ask_more) {
+          ask = item_of(ask_id);
+          describe();
+        }
+      }
+    };
+    auto ask_stage = [&]() {
+      const unsigned k0 = ask_k0(), ow = ask_in_k() ? vw : kBufOob, ox = ask_in_k() ? vx : kBufOob;
 #pragma unroll
-      for (int p = 0; p < PW + PX; ++p) issue_piece(s, p, ow, ox);
-    };
-    auto wait_stage = [&](int newer) {  // this wave's pieces of all but the newest `newer` stages have landed
-      if (newer >= 2 && NBUF > 3) wait_dma_all_but<2 * (PW + PX)>();
-      else if (newer >= 1) wait_dma_all_but<PW + PX>();
-      else wait_dma_all_but<0>();
+      for (int p = 0; p < 2 * PW; ++p) ask_piece(p, k0, ow, ox);
+      ask_next();
     };
     // One half stage: the products of fragment set `slot`; between those of its first half the other set's fragments are read
-    // (k-step `ks` of buffer `buf`), between the rest, where `more`, the DMA pieces of stage s + NBUF are issued: the
-    // matrix unit works on meanwhile, and a fragment has half of the products' time to arrive.
-    auto half_stage = [&](auto slot_c, const uint4* buf, int ks, auto more_c, int s) {
+    // (k-step `ks` of buffer `buf`), between the rest of the second half stage the DMA pieces of the next asked stage are
+    // issued: the matrix unit works on meanwhile, and a fragment has half of the products' time to arrive.
+    auto half_stage = [&](auto slot_c, auto last_c, const uint4* buf, int ks) {
       constexpr int slot = decltype(slot_c)::value;
-      constexpr bool more = decltype(more_c)::value;
-      constexpr int NP = TN * TM, NR = TN + TM;
-      unsigned ow = 0, ox = 0;
-      if constexpr (more) { ow = in_k(s + NBUF) ? vw : kBufOob; ox = in_k(s + NBUF) ? vx : kBufOob; }
+      constexpr bool last = decltype(last_c)::value;       // products only
+      constexpr bool more = slot == 1 && !last;
+      unsigned k0 = 0, ow = 0, ox = 0;
+      if constexpr (more) { k0 = ask_k0(); ow = ask_in_k() ? vw : kBufOob; ox = ask_in_k() ? vx : kBufOob; }
       static_for<NP>([&](auto qc) {
-        constexpr int q = decltype(qc)::value, i = q / TM, j = q % TM;
+        constexpr int q = decltype(qc)::value, i = q / TW, j = q % TW;
         acc[i][j] = mfma_32x32x32_i8(wf[slot][i], xf[slot][j], acc[i][j]);
         sched_fence();
-        if (buf) {
-          constexpr int r0 = 2 * q * NR / NP < NR ? 2 * q * NR / NP : NR, r1 = 2 * (q + 1) * NR / NP < NR ? 2 * (q + 1) * NR / NP : NR;
+        constexpr int r0 = 2 * q * NR / NP < NR ? 2 * q * NR / NP : NR, r1 = 2 * (q + 1) * NR / NP < NR ? 2 * (q + 1) * NR / NP : NR;
+        if constexpr (!last) {
 #pragma unroll
           for (int r = r0; r < r1; ++r) read_frag(slot ^ 1, buf, ks, r);
         }
         if constexpr (more) {
-          constexpr int h = NP / 2, p0 = q < h ? 0 : (q - h) * (PW + PX) / (NP - h), p1 = q < h ? 0 : (q + 1 - h) * (PW + PX) / (NP - h);
+          constexpr int h = NP / 2, n = NP - h;
+          constexpr int p0 = q < h ? 0 : (q - h) * 2 * PW / n, p1 = q < h ? 0 : (q + 1 - h) * 2 * PW / n;
 #pragma unroll
-          for (int p = p0; p < p1; ++p) issue_piece(s + NBUF, p, ow, ox);
+          for (int p = p0; p < p1; ++p) ask_piece(p, k0, ow, ox);
         }
         sched_fence();
       });
+      if constexpr (more) ask_next();
     };
-    for (int s = 0; s < NBUF - 1 && s < ns; ++s) issue(s);
-    wait_stage((ns < NBUF - 1 ? ns : NBUF - 1) - 1);
-    wg_barrier_nodrain();
-    // one more stage ahead than in the loop: buffer NBUF - 1 is still empty
-    if (NBUF - 1 < ns) issue(NBUF - 1);
-#pragma unroll
-    for (int r = 0; r < TN + TM; ++r) read_frag(0, lds, 0, r);
     constexpr std::integral_constant<int, 0> c0{};
     constexpr std::integral_constant<int, 1> c1{};
     constexpr std::false_type no{};
     constexpr std::true_type yes{};
-    int s = 0;
-    for (; s + NBUF < ns; ++s) {
-      half_stage(c0, lds + (s % NBUF) * STAGE, 1, no, 0);
-      wait_lds_reads();                                  // this wave's fragments of stage s are in registers
-      wait_dma_all_but<(NBUF - 2) * (PW + PX)>();        // stages s+1 .. s+NBUF-1 are in flight: s+1 has landed
-      wg_barrier_nodrain();
-      half_stage(c1, lds + ((s + 1) % NBUF) * STAGE, 0, yes, s);   // stage s+NBUF into the buffer that stage s leaves
+
+    describe();
+    for (int q = 0; q < NBUF; ++q) ask_stage();      // (every buffer is empty)
+    wait_dma_all_but<(NBUF - 1) * 2 * PW>();
+    wg_barrier_nodrain();
+#pragma unroll
+    for (int r = 0; r < NR; ++r) read_frag(0, lds, 0, r);
+    int g = 0;                          // stages taken; asked = g + NBUF up to the middle of a stage
+    for (int tile = 0;; ++tile) {
+      for (int s = 0; s < cur.ns - (BIG ? 1 : 0); ++s, ++g) {
+        half_stage(c0, no, lds + (g % NBUF) * STAGE, 1);
+        wait_lds_reads();               // this wave's fragments of stage g are in registers
+        // stage g + 1 has landed (stores and parameter pieces among the newer operations only make the wait stricter)
+        wait_dma_all_but<(NBUF - 2) * 2 * PW>();
+        wg_barrier_nodrain();
+        half_stage(c1, no, lds + ((g + 1) % NBUF) * STAGE, 0);  // asks into the buffer that stage g leaves
+      }
+      if constexpr (BIG) {              // (the sums leave their accumulators from the block that finishes them)
+        half_stage(c0, no, lds + (g % NBUF) * STAGE, 1);
+        half_stage(c1, yes, lds, 0);
+      }
+      finish(cur, params + (tile % 3) * SLOT);
+      if constexpr (BIG) break;
+      id += gx;
+      if (id >= xend) break;
+      cur = item_of(id);
+      clear();
     }
-    for (; s + 1 < ns; ++s) {
-      half_stage(c0, lds + (s % NBUF) * STAGE, 1, no, 0);
-      wait_lds_reads();
-      wait_stage(ns - 1 - (s + 1));
-      wg_barrier_nodrain();
-      half_stage(c1, lds + ((s + 1) % NBUF) * STAGE, 0, no, 0);
-    }
-    half_stage(c0, lds + (s % NBUF) * STAGE, 1, no, 0);
-    half_stage(c1, nullptr, 0, no, 0);
+    wait_dma_all_but<0>();              // (the stages behind the end write zeros into this workgroup's LDS)
   } else {
+    for (int c = tid; c < B; c += 256) {
+      const int ch = cur.n0 + c < a.n ? cur.n0 + c : a.n - 1;
+      params[c] = ld(a.sw + ch);
+      params[B + c] = a.bias ? ld(a.bias + ch) : 0.0f;
+      params[2 * B + c] = ld(a.sx + (cur.m0 + c < a.m ? cur.m0 + c : a.m - 1));
+    }
     constexpr int CH = STAGE / 256;       // chunks of a thread per stage
-    constexpr int AHEAD = BM * BN > 64 * 64 ? 2 : 4;   // stages in registers
+    constexpr int AHEAD = B > 64 ? 2 : 4;   // stages in registers
     uint4 q[AHEAD][CH];
     auto fetch = [&](int s, uint4 (&to)[CH]) {
-      const int k0 = (s_begin + s) * 64;
+      const int k0 = (cur.s_begin + s) * 64;
 #pragma unroll
       for (int p = 0; p < CH; ++p) {
         const int id4 = p * 256 + tid, row = id4 >> 2, at = k0 + (id4 & 3) * 16;
         to[p] = make_uint4(0u, 0u, 0u, 0u);
-        if (row < BN) { if (n0 + row < a.n) to[p] = i8_chunk(a.w + (long)(n0 + row) * a.ldw, at, a.k); }
-        else if (m0 + row - BN < a.m) to[p] = i8_chunk(a.x + (m0 + row - BN) * a.ldx, at, a.k);
+        if (row < B) { if (cur.n0 + row < a.n) to[p] = i8_chunk(a.w + (long)(cur.n0 + row) * a.ldw, at, a.k); }
+        else if (cur.m0 + row - B < a.m) to[p] = i8_chunk(a.x + (cur.m0 + row - B) * a.ldx, at, a.k);
       }
     };
-    static_for<AHEAD>([&](auto d) { if (decltype(d)::value < ns) fetch(decltype(d)::value, q[decltype(d)::value]); });
-    for (int s0 = 0; s0 < ns; s0 += AHEAD)
+    static_for<AHEAD>([&](auto d) { if (decltype(d)::value < cur.ns) fetch(decltype(d)::value, q[decltype(d)::value]); });
+    for (int s0 = 0; s0 < cur.ns; s0 += AHEAD)
       static_for<AHEAD>([&](auto d) {
         constexpr int v = decltype(d)::value;
         const int s = s0 + v;
-        if (s < ns) {
+        if (s < cur.ns) {
           uint4* const buf = lds + (s & 1) * STAGE;
 #pragma unroll
           for (int p = 0; p < CH; ++p) {
             const int id4 = p * 256 + tid, row = id4 >> 2;
-            buf[row * 4 + ((id4 & 3) ^ ((row >> 1) & 3))] = q[v][p];
+            buf[row * 4 + ((id4 & 3) ^ ((row >> 2) & 3))] = q[v][p];
           }
-          if (s + AHEAD < ns) fetch(s + AHEAD, q[v]);
+          if (s + AHEAD < cur.ns) fetch(s + AHEAD, q[v]);
           // (one barrier a stage: a wave may write buffer s+1 -- last read in stage s-1 -- while others still read buffer s)
           wait_lds_reads();
           wg_barrier_nodrain();
 #pragma unroll
           for (int ks = 0; ks < 2; ++ks) {
 #pragma unroll
-            for (int r = 0; r < TN + TM; ++r) read_frag(0, buf, ks, r);
+            for (int r = 0; r < NR; ++r) read_frag(0, buf, ks, r);
 #pragma unroll
-            for (int i = 0; i < TN; ++i)
+            for (int i = 0; i < TW; ++i)
 #pragma unroll
-              for (int j = 0; j < TM; ++j) acc[i][j] = mfma_32x32x32_i8(wf[0][i], xf[0][j], acc[i][j]);
+              for (int j = 0; j < TW; ++j) acc[i][j] = mfma_32x32x32_i8(wf[0][i], xf[0][j], acc[i][j]);
           }
         }
       });
-  }
-
-  // ---- epilogue: a lane holds row m0 + wm + 32 j + l31 and channels 8 q + 4 half + {0..3}, q = 0..3, of each 32-channel block
-  if (!BIG && a.ksplit > 1) {
-#pragma unroll
-    for (int j = 0; j < TM; ++j) {
-      const long row = m0 + wm + 32 * j + l31;
-      if (row < a.m) {
-        int* const to = a.part + ((long)slice * a.m + row) * a.n;
-#pragma unroll
-        for (int i = 0; i < TN; ++i)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int ch = n0 + wn + 32 * i + (r & 3) + 8 * (r >> 2) + 4 * half;
-            if (ch < a.n) st(to + ch, acc[i][j][r]);
-          }
-      }
-    }
-    return;
-  }
-  float sx[TM];
-#pragma unroll
-  for (int j = 0; j < TM; ++j) {
-    const long row = m0 + wm + 32 * j + l31;
-    sx[j] = ld(a.sx + (row < a.m ? row : a.m - 1));      // (rows and channels behind the last: any value, never stored)
-  }
-#pragma unroll
-  for (int i = 0; i < TN; ++i) {
-    float sw[16], bias[16];
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      int ch = n0 + wn + 32 * i + (r & 3) + 8 * (r >> 2) + 4 * half;
-      ch = ch < a.n ? ch : a.n - 1;
-      sw[r] = ld(a.sw + ch);
-      bias[r] = a.bias ? ld(a.bias + ch) : 0.0f;
-    }
-#pragma unroll
-    for (int j = 0; j < TM; ++j) {
-      const long row = m0 + wm + 32 * j + l31;
-      T* const yr = (T*)a.y + row * a.ldy;
-      float v[16];
-#pragma unroll
-      for (int r = 0; r < 16; ++r) v[r] = (float)acc[i][j][r] * sx[j] * sw[r] + bias[r];
-      if (a.act != ECO_ACT_NONE) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) v[r] = i8_activate(v[r], a.act);
-      }
-      if (BIG || a.vec) {
-        // two groups of four channels per lane pair -> eight consecutive channels in one lane
-#pragma unroll
-        for (int q = 0; q < 4; q += 2) {
-          const int ch = n0 + wn + 32 * i + 8 * (q + half);
-          if constexpr (sizeof(T) == 2) {
-            unsigned lo[2] = {pack_bf16x2(v[4 * q], v[4 * q + 1]), pack_bf16x2(v[4 * q + 2], v[4 * q + 3])};
-            unsigned hi[2] = {pack_bf16x2(v[4 * q + 4], v[4 * q + 5]), pack_bf16x2(v[4 * q + 6], v[4 * q + 7])};
-            permlane32_swap(lo[0], hi[0]);
-            permlane32_swap(lo[1], hi[1]);
-            if (row < a.m && ch < a.n) st((uint4*)(yr + ch), make_uint4(lo[0], lo[1], hi[0], hi[1]));
-          } else {
-            unsigned lo[4], hi[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              lo[e] = f32_bits(v[4 * q + e]);
-              hi[e] = f32_bits(v[4 * q + 4 + e]);
-              permlane32_swap(lo[e], hi[e]);
-            }
-            if (row < a.m && ch < a.n) {
-              st((uint4*)(yr + ch), make_uint4(lo[0], lo[1], lo[2], lo[3]));
-              st((uint4*)(yr + ch + 4), make_uint4(hi[0], hi[1], hi[2], hi[3]));
-            }
-          }
-        }
-      } else if (row < a.m) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int ch = n0 + wn + 32 * i + (r & 3) + 8 * (r >> 2) + 4 * half;
-          if (ch < a.n) i8_store(yr + ch, v[r]);
-        }
-      }
-    }
+    finish(cur, params);
   }
 }
 
@@ -460,14 +537,16 @@ static inline unsigned i8_grid(long count, long per_block) {
 
 constexpr int kTokMax = 32;     // rows up to which the token kernel is taken
 
-template <int BM, int BN, int WM, int WN, int NBUF, bool FAST, typename T>
-static int i8_launch_tile(I8Args& a, hipStream_t st) {
-  a.tiles_m = (int)ceil_div(a.m, BM);
-  a.tiles_n = (int)ceil_div(a.n, BN);
-  const int bufs = FAST ? (a.nstages < NBUF ? a.nstages : NBUF) : 2;
-  ECO_RAISE_DYNAMIC_LDS((i8_tile_kernel<BM, BN, WM, WN, NBUF, FAST, T>), "inner_product_i8");
-  hipLaunchKernelGGL((i8_tile_kernel<BM, BN, WM, WN, NBUF, FAST, T>), dim3((unsigned)(a.tiles_m * a.tiles_n * a.ksplit)),
-                     dim3(kI8Threads), (unsigned)(bufs * (BM + BN) * 64), st, a);
+template <int B, int NBUF, bool FAST, typename T>
+static int i8_launch_tile(I8Args& a, int num_cu, hipStream_t st) {
+  a.tiles_m = (int)ceil_div(a.m, B);
+  a.tiles_n = (int)ceil_div(a.n, B);
+  const long total = (long)a.tiles_m * a.tiles_n * a.ksplit;
+  constexpr int kLds = NBUF * 2 * B * 64 + 3 * 3 * B * 4;
+  constexpr int kPerCu = B > 128 ? 1 : B > 64 ? 3 : 6;     // workgroups that a compute unit's 160 KB of LDS hold
+  const long grid = FAST && B <= 128 && total > (long)kPerCu * num_cu ? (long)kPerCu * num_cu : total;
+  ECO_RAISE_DYNAMIC_LDS((i8_tile_kernel<B, NBUF, FAST, T>), "inner_product_i8");
+  hipLaunchKernelGGL((i8_tile_kernel<B, NBUF, FAST, T>), dim3((unsigned)grid), dim3(kI8Threads), (unsigned)kLds, st, a);
   if (int rc = check_launch("eco_inner_product_i8_forward")) return rc;
   if (a.ksplit > 1) {
     hipLaunchKernelGGL((i8_join_kernel<T>), dim3(i8_grid(a.m * a.n, kI8Threads)), dim3(kI8Threads), 0, st, a);
@@ -490,12 +569,12 @@ static int i8_launch(const eco_inner_product_i8_plan& p, I8Args& a, bool fast, h
     return check_launch("eco_inner_product_i8_forward(tokens)");
   }
   if (fast) {
-    if (p.bm == 256 && a.vec) return i8_launch_tile<256, 256, 128, 128, 4, true, T>(a, st);
-    if (p.bm >= 128) return i8_launch_tile<128, 128, 64, 64, 3, true, T>(a, st);
-    return i8_launch_tile<64, 64, 32, 32, 3, true, T>(a, st);
+    if (p.bm == 256 && a.vec) return i8_launch_tile<256, 4, true, T>(a, p.num_cu, st);
+    if (p.bm >= 128) return i8_launch_tile<128, 3, true, T>(a, p.num_cu, st);
+    return i8_launch_tile<64, 3, true, T>(a, p.num_cu, st);
   }
-  if (p.bm >= 128) return i8_launch_tile<128, 128, 64, 64, 3, false, T>(a, st);
-  return i8_launch_tile<64, 64, 32, 32, 3, false, T>(a, st);
+  if (p.bm >= 128) return i8_launch_tile<128, 2, false, T>(a, p.num_cu, st);
+  return i8_launch_tile<64, 2, false, T>(a, p.num_cu, st);
 }
 
 }  // namespace eco

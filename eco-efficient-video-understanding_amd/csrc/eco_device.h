@@ -69,6 +69,31 @@ __device__ __forceinline__ i32x4 mfma_16x16x64_i8(uint4 a, uint4 b, i32x4 c) {
 #endif
 }
 
+// The same, accumulating in place in four accumulator registers (AGPRs).  With the builtin the allocator may give result and
+// addend different registers, and for a wave whose sums fill the accumulator file it then moved sums around in the loop.
+// The compiler pads no hazard of an asm statement: the sums must not be touched by another instruction until
+// agpr_sums_settled() -- between their last product and a read, between their setting and the first product --, and
+// fragments come from LDS reads (whose arrival the compiler waits for), not from instructions just ahead.
+__device__ __forceinline__ void mfma_16x16x64_i8_agpr(i32x4& c, uint4 a, uint4 b) {
+#ifdef ECO_EMU
+  c = emu::mfma_i32_16x16x64_i8(a, b, c);
+#else
+  asm volatile("v_mfma_i32_16x16x64_i8 %0, %1, %2, %0" : "+a"(c) : "v"(__builtin_bit_cast(i32x4, a)), "v"(__builtin_bit_cast(i32x4, b)));
+#endif
+}
+__device__ __forceinline__ void agpr_sums_settled() {
+#ifndef ECO_EMU
+  asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
+#endif
+}
+
+// Ties a sum to the place behind agpr_sums_settled(): later reads use this statement's result.
+#ifdef ECO_EMU
+#define ECO_AFTER_SETTLED(v) ((void)(v))
+#else
+#define ECO_AFTER_SETTLED(v) asm volatile("" : "+a"(v))
+#endif
+
 // fp32 <-> bf16 (round to nearest even; the GPU form is v_cvt_pk_bf16_f32, the expression below gives the same
 // bits for every finite input and for infinities).
 __device__ __forceinline__ unsigned f32_to_bf16_bits(float f) {
@@ -221,6 +246,21 @@ __device__ __forceinline__ void permlane32_swap(unsigned& a, unsigned& b) {
   memcpy(&a, &na, 4); memcpy(&b, &nb, 4);
 #else
   const auto r = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+  a = r[0]; b = r[1];
+#endif
+}
+
+// v_permlane16_swap: rows of sixteen lanes; row 1 of a trades places with row 0 of b, row 3 of a with row 2 of b.
+__device__ __forceinline__ void permlane16_swap(unsigned& a, unsigned& b) {
+#ifdef ECO_EMU
+  const int l = emu::tls_cur->lane;
+  float fa, fb;
+  memcpy(&fa, &a, 4); memcpy(&fb, &b, 4);
+  const float xa = emu::wave_xchg_f32(fa, l ^ 16), xb = emu::wave_xchg_f32(fb, l ^ 16);
+  const float na = l & 16 ? xb : fa, nb = l & 16 ? fb : xa;
+  memcpy(&a, &na, 4); memcpy(&b, &nb, 4);
+#else
+  const auto r = __builtin_amdgcn_permlane16_swap(a, b, false, false);
   a = r[0]; b = r[1];
 #endif
 }

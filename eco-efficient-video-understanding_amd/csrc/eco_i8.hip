@@ -182,29 +182,31 @@ __global__ __launch_bounds__(512) void i8_token_kernel(const I8Args a) {
 }
 
 // ---- tiles on the matrix cores -------------------------------------------------------------------------------------------------
-// A workgroup of four waves takes B output channels x B rows, each wave W x W of them (W = B / 2) as 32x32 products (D's rows are
-// channels, so that a lane ends up with consecutive channels of one row of y).  Both operands pass through LDS in stages of
-// 64 bytes of k, rows 64 bytes apart, the four 16-byte chunks of row r stored in the order c ^ ((r >> 2) & 3): sixteen lanes
-// that read a fragment then touch all 64 banks once.
+// A workgroup of four waves takes B output channels x B rows, each wave W x W of them (W = B / 2) as 16x16 products over 64 bytes
+// of k (D's rows are channels, so that a lane ends up with consecutive channels of one row of y).  16x16x64 rather than
+// 32x32x32: the same rate, half the accumulator traffic a product -- and this kernel runs at the clock that its power allows.
+// Both operands pass through LDS in stages of 64 bytes of k, rows 64 bytes apart, the four 16-byte chunks of row r stored in
+// the order c ^ (-(r >> 2) & 3): the sixteen lanes that a fragment's 16-byte read serves at once (0-3, 12-15, 20-23, 24-27,
+// then the others) touch all 64 banks once.  A wave holds a stage's
+// fragments in registers, twice: the next stage's are read while this one's products run.
 //   FAST  (rows on 16-byte boundaries, k a multiple of 16): persistent workgroups walk their tiles' stages as ONE stream through
-//         NBUF buffers filled by LDS-DMA, up to NBUF stages ahead -- across the ends of tiles, so that a tile's stores
-//         run under the next one's loads.  (The 256 tile's sums fill the accumulator file, fragments held across its end
-//         spill: one tile a workgroup.)  A buffer is refilled behind the barrier in the middle of its own stage, when every
-//         wave has its last fragments in registers.  A tile's scales and bias come the same way, into one of three slots.
+//         NBUF buffers filled by LDS-DMA -- across the ends of tiles, so that a tile's stores run under the next one's loads.
+//         (The 256 tile's sums fill the accumulator file, fragments held across its end would spill: one tile a workgroup.)
+//         One barrier a stage: behind it the next stage has landed, and the buffer of this one -- every wave has its
+//         fragments -- is refilled.  A tile's scales and bias come the same way, into one of three slots.
 //   else  any alignment: one tile a workgroup, operands through registers
 template <int B, int NBUF, bool FAST, typename T>
 __global__ __launch_bounds__(256, B > 128 ? 1 : 3) void i8_tile_kernel(const I8Args a) {
-  constexpr int W = B / 2, TW = W / 32;                  // TW x TW products of 32x32 a wave
+  constexpr int W = B / 2, TW = W / 16;                  // TW x TW products of 16x16 a wave
   constexpr bool BIG = B > 128;                          // (taken with whole sums and 16-byte stores only)
   constexpr int STAGE = 2 * B * 4;                       // 16-byte vectors of a stage: B rows of w, then B rows of x
-  constexpr int NR = 2 * TW, NP = TW * TW;               // fragments and products of a k-step
+  constexpr int NR = 2 * TW, NP = TW * TW;               // fragments and products of a stage
   constexpr int PW = B / 64;                             // DMA pieces (16 rows x 64 bytes) of a wave per stage and operand
   constexpr int SLOT = 3 * B;                            // floats of a tile's parameters: sw, bias, sx
   ECO_DYNAMIC_LDS(lds_f);
   uint4* const lds = (uint4*)lds_f;
   float* const params = lds_f + NBUF * STAGE * 4;
   const int tid = (int)threadIdx.x, lane = lane_id(), wave = uniform(tid >> 6);
-  const int half = lane >> 5, l31 = lane & 31;
   const int wn = (wave & 1) * W, wm = (wave >> 1) * W;
 
   // Tile numbers: XCD b % 8 owns a contiguous range, its workgroups take every gx-th of it; inside, groups of eight row tiles
@@ -215,7 +217,7 @@ __global__ __launch_bounds__(256, B > 128 ? 1 : 3) void i8_tile_kernel(const I8A
   const int xend = xbase + (total >> 3) + (xcd < (total & 7) ? 1 : 0);
   struct Item {
     long m0;
-    int n0, slice, s_begin, ns;
+    int n0, slice, s_begin, s_end, ns;
   };
   auto item_of = [&](int id) {
     Item t;
@@ -228,47 +230,52 @@ __global__ __launch_bounds__(256, B > 128 ? 1 : 3) void i8_tile_kernel(const I8A
     t.n0 = uniform(q * B);
     t.slice = uniform(t.slice);
     t.s_begin = uniform(a.nstages * t.slice / a.ksplit);              // (at most 2048 stages, 16 slices)
-    // (two stages at least: a tile's parameters are asked for at most two tiles ahead; the stage behind k is zeros)
-    const int ns = uniform(a.nstages * (t.slice + 1) / a.ksplit) - t.s_begin;
-    t.ns = ns < 2 ? 2 : ns;
+    // (an even number of stages, for the two fragment sets; a stage behind the slice's end is zeros)
+    t.s_end = uniform(a.nstages * (t.slice + 1) / a.ksplit);
+    t.ns = (t.s_end - t.s_begin + 1) & ~1;
     return t;
   };
 
-  i32x16 acc[TW][TW];
+  i32x4 acc[TW][TW];
   auto clear = [&]() {
 #pragma unroll
     for (int i = 0; i < TW; ++i)
 #pragma unroll
-      for (int j = 0; j < TW; ++j)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) acc[i][j][r] = 0;
+      for (int j = 0; j < TW; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
   };
   uint4 wf[2][TW], xf[2][TW];
-  // fragment r of k-step ks (r < TW: w's, else x's)
-  const int fsw = (l31 >> 2) & 3, fw = (wn + l31) * 4, fx = (B + wm + l31) * 4;
-  const int fk[2] = {half ^ fsw, (2 + half) ^ fsw};
-  auto read_frag = [&](int slot, const uint4* buf, int ks, int r) {
-    if (r < TW) wf[slot][r] = buf[fw + fk[ks] + 128 * r];
-    else xf[slot][r - TW] = buf[fx + fk[ks] + 128 * (r - TW)];
+  // fragment r of a stage (r < TW: w's, else x's)
+  const int fk = (lane >> 4) ^ (-(lane >> 2) & 3);
+  const int fw = (wn + (lane & 15)) * 4 + fk, fx = (B + wm + (lane & 15)) * 4 + fk;
+  auto read_frag = [&](int slot, const uint4* buf, int r) {
+    if (r < TW) wf[slot][r] = buf[fw + 64 * r];
+    else xf[slot][r - TW] = buf[fx + 64 * (r - TW)];
   };
 
-  // A lane holds row m0 + wm + 32 j + l31 and channels 8 q + 4 half + {0..3}, q = 0..3, of each 32-channel block.
+  // A lane holds row m0 + wm + 16 j + (lane & 15) and channels 4 (lane >> 4) + {0..3} of each 16-channel block.
   auto finish = [&](const Item& t, const float* par) {
     // (opaque per tile: as invariants of the tile loop their many addresses would be computed once and live in scratch memory)
-    int l31 = lane & 31, half = lane >> 5;
-    ECO_OPAQUE(l31);
-    ECO_OPAQUE(half);
+    if constexpr (BIG) {
+      agpr_sums_settled();
+#pragma unroll
+      for (int i = 0; i < TW; ++i)
+#pragma unroll
+        for (int j = 0; j < TW; ++j) ECO_AFTER_SETTLED(acc[i][j]);
+    }
+    int l15 = lane & 15, l4 = lane >> 4;
+    ECO_OPAQUE(l15);
+    ECO_OPAQUE(l4);
     if (!BIG && a.ksplit > 1) {
 #pragma unroll
       for (int j = 0; j < TW; ++j) {
-        const long row = t.m0 + wm + 32 * j + l31;
+        const long row = t.m0 + wm + 16 * j + l15;
         if (row < a.m) {
           int* const to = a.part + ((long)t.slice * a.m + row) * a.n;
 #pragma unroll
           for (int i = 0; i < TW; ++i)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-              const int ch = t.n0 + wn + 32 * i + (r & 3) + 8 * (r >> 2) + 4 * half;
+            for (int r = 0; r < 4; ++r) {
+              const int ch = t.n0 + wn + 16 * i + 4 * l4 + r;
               if (ch < a.n) st(to + ch, acc[i][j][r]);
             }
         }
@@ -277,66 +284,60 @@ __global__ __launch_bounds__(256, B > 128 ? 1 : 3) void i8_tile_kernel(const I8A
     }
     float sx[TW];
 #pragma unroll
-    for (int j = 0; j < TW; ++j) sx[j] = par[2 * B + wm + 32 * j + l31];
+    for (int j = 0; j < TW; ++j) sx[j] = par[2 * B + wm + 16 * j + l15];
 #pragma unroll
-    for (int i = 0; i < TW; ++i) {
+    for (int i = 0; i < TW; i += 2) {
       sched_fence();          // (one block's parameters in registers at a time)
-      float4 sw[4], bias[4];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        sw[q] = *(const float4*)(par + wn + 32 * i + 8 * q + 4 * half);
-        bias[q] = *(const float4*)(par + B + wn + 32 * i + 8 * q + 4 * half);
-      }
+      const float4 sw0 = *(const float4*)(par + wn + 16 * i + 4 * l4), sw1 = *(const float4*)(par + wn + 16 * i + 16 + 4 * l4);
+      const float4 b0 = *(const float4*)(par + B + wn + 16 * i + 4 * l4), b1 = *(const float4*)(par + B + wn + 16 * i + 16 + 4 * l4);
 #pragma unroll
       for (int j = 0; j < TW; ++j) {
         sched_fence();
-        const long row = t.m0 + wm + 32 * j + l31;
+        const long row = t.m0 + wm + 16 * j + l15;
         T* const yr = (T*)a.y + row * a.ldy;
-        float v[16];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const i32x16& c = acc[i][j];
-          v[4 * q] = (float)c[4 * q] * sx[j] * sw[q].x + bias[q].x;
-          v[4 * q + 1] = (float)c[4 * q + 1] * sx[j] * sw[q].y + bias[q].y;
-          v[4 * q + 2] = (float)c[4 * q + 2] * sx[j] * sw[q].z + bias[q].z;
-          v[4 * q + 3] = (float)c[4 * q + 3] * sx[j] * sw[q].w + bias[q].w;
-        }
+        const i32x4 c0 = acc[i][j], c1 = acc[i + 1][j];
+        float v[8];
+        v[0] = (float)c0[0] * sx[j] * sw0.x + b0.x;
+        v[1] = (float)c0[1] * sx[j] * sw0.y + b0.y;
+        v[2] = (float)c0[2] * sx[j] * sw0.z + b0.z;
+        v[3] = (float)c0[3] * sx[j] * sw0.w + b0.w;
+        v[4] = (float)c1[0] * sx[j] * sw1.x + b1.x;
+        v[5] = (float)c1[1] * sx[j] * sw1.y + b1.y;
+        v[6] = (float)c1[2] * sx[j] * sw1.z + b1.z;
+        v[7] = (float)c1[3] * sx[j] * sw1.w + b1.w;
         if (a.act == ECO_ACT_RELU) {
 #pragma unroll
-          for (int r = 0; r < 16; ++r) v[r] = i8_activate(v[r], ECO_ACT_RELU);
+          for (int r = 0; r < 8; ++r) v[r] = i8_activate(v[r], ECO_ACT_RELU);
         } else if (a.act == ECO_ACT_SILU) {
 #pragma unroll
-          for (int r = 0; r < 16; ++r) v[r] = i8_activate(v[r], ECO_ACT_SILU);
+          for (int r = 0; r < 8; ++r) v[r] = i8_activate(v[r], ECO_ACT_SILU);
         }
         if (BIG || a.vec) {
-          // two groups of four channels per lane pair -> eight consecutive channels in one lane
+          // four channels of each of two blocks -> eight consecutive ones: lane rows 0..3 end up with channels 0, 16, 8, 24 on
+          const int ch = t.n0 + wn + 16 * i + 16 * (l4 & 1) + 4 * (l4 & 2);
+          if constexpr (sizeof(T) == 2) {
+            unsigned lo[2] = {pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+            unsigned hi[2] = {pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])};
+            permlane16_swap(lo[0], hi[0]);
+            permlane16_swap(lo[1], hi[1]);
+            if (row < a.m && ch < a.n) st((uint4*)(yr + ch), make_uint4(lo[0], lo[1], hi[0], hi[1]));
+          } else {
+            unsigned lo[4], hi[4];
 #pragma unroll
-          for (int q = 0; q < 4; q += 2) {
-            const int ch = t.n0 + wn + 32 * i + 8 * (q + half);
-            if constexpr (sizeof(T) == 2) {
-              unsigned lo[2] = {pack_bf16x2(v[4 * q], v[4 * q + 1]), pack_bf16x2(v[4 * q + 2], v[4 * q + 3])};
-              unsigned hi[2] = {pack_bf16x2(v[4 * q + 4], v[4 * q + 5]), pack_bf16x2(v[4 * q + 6], v[4 * q + 7])};
-              permlane32_swap(lo[0], hi[0]);
-              permlane32_swap(lo[1], hi[1]);
-              if (row < a.m && ch < a.n) st((uint4*)(yr + ch), make_uint4(lo[0], lo[1], hi[0], hi[1]));
-            } else {
-              unsigned lo[4], hi[4];
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                lo[e] = f32_bits(v[4 * q + e]);
-                hi[e] = f32_bits(v[4 * q + 4 + e]);
-                permlane32_swap(lo[e], hi[e]);
-              }
-              if (row < a.m && ch < a.n) {
-                st((uint4*)(yr + ch), make_uint4(lo[0], lo[1], lo[2], lo[3]));
-                st((uint4*)(yr + ch + 4), make_uint4(hi[0], hi[1], hi[2], hi[3]));
-              }
+            for (int e = 0; e < 4; ++e) {
+              lo[e] = f32_bits(v[e]);
+              hi[e] = f32_bits(v[4 + e]);
+              permlane16_swap(lo[e], hi[e]);
+            }
+            if (row < a.m && ch < a.n) {
+              st((uint4*)(yr + ch), make_uint4(lo[0], lo[1], lo[2], lo[3]));
+              st((uint4*)(yr + ch + 4), make_uint4(hi[0], hi[1], hi[2], hi[3]));
             }
           }
         } else if (row < a.m) {
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int ch = t.n0 + wn + 32 * i + (r & 3) + 8 * (r >> 2) + 4 * half;
+          for (int r = 0; r < 8; ++r) {
+            const int ch = t.n0 + wn + 16 * i + 16 * (r >> 2) + 4 * l4 + (r & 3);
             if (ch < a.n) i8_store(yr + ch, v[r]);
           }
         }
@@ -349,7 +350,7 @@ __global__ __launch_bounds__(256, B > 128 ? 1 : 3) void i8_tile_kernel(const I8A
   Item cur = item_of(id);
 
   if constexpr (FAST) {
-    const int prow = lane >> 2, pchunk = (lane & 3) ^ (prow >> 2);
+    const int prow = lane >> 2, pchunk = (lane & 3) ^ (-(prow >> 2) & 3);
     const unsigned vw = (unsigned)((long)prow * a.ldw + pchunk * 16), vx = (unsigned)((long)prow * a.ldx + pchunk * 16);
     const unsigned ldw16 = (unsigned)(16 * a.ldw), ldx16 = (unsigned)(16 * a.ldx);
     // ---- the asking side of the stream: item, stage in it, its operands' descriptors (from the tile's first row to the
@@ -378,14 +379,14 @@ __global__ __launch_bounds__(256, B > 128 ? 1 : 3) void i8_tile_kernel(const I8A
 #endif
     };
     // piece p (0 .. 2 PW - 1: w's, then x's) of the stage that is asked for next
-    auto ask_piece = [&](int p, unsigned k0, unsigned ow, unsigned ox) {
+    auto ask_piece = [&](int p, unsigned k0, unsigned off) {
       uint4* const buf = lds + (asked % NBUF) * STAGE;
-      if (p < PW) glds16_buf(rw, ow, k0 + (unsigned)(p * 4 + wave) * ldw16, buf + (p * 4 + wave) * 64);
-      else glds16_buf(rx, ox, k0 + (unsigned)((p - PW) * 4 + wave) * ldx16, buf + B * 4 + ((p - PW) * 4 + wave) * 64);
+      if (p < PW) glds16_buf(rw, off, k0 + (unsigned)(p * 4 + wave) * ldw16, buf + (p * 4 + wave) * 64);
+      else glds16_buf(rx, off, k0 + (unsigned)((p - PW) * 4 + wave) * ldx16, buf + B * 4 + ((p - PW) * 4 + wave) * 64);
     };
     auto ask_k0 = [&]() { return (unsigned)((ask.s_begin + ask_s) * 64); };
     // (chunks behind k, and the stages asked for behind the stream's end: zeros, nothing is read)
-    auto ask_in_k = [&]() { return ask_more && (int)ask_k0() + pchunk * 16 < a.k; };
+    auto ask_in_k = [&]() { return ask_more && ask.s_begin + ask_s < ask.s_end && (int)ask_k0() + pchunk * 16 < a.k; };
     auto ask_next = [&]() {             // one stage further
       ++asked;
       if (++ask_s == ask.ns && ask_more) {
@@ -399,67 +400,67 @@ __global__ __launch_bounds__(256, B > 128 ? 1 : 3) void i8_tile_kernel(const I8A
         }
       }
     };
-    auto ask_stage = [&]() {
-      const unsigned k0 = ask_k0(), ow = ask_in_k() ? vw : kBufOob, ox = ask_in_k() ? vx : kBufOob;
-#pragma unroll
-      for (int p = 0; p < 2 * PW; ++p) ask_piece(p, k0, ow, ox);
-      ask_next();
-    };
-    // One half stage: the products of fragment set `slot`; between those of its first half the other set's fragments are read
-    // (k-step `ks` of buffer `buf`), between the rest of the second half stage the DMA pieces of the next asked stage are
-    // issued: the matrix unit works on meanwhile, and a fragment has half of the products' time to arrive.
-    auto half_stage = [&](auto slot_c, auto last_c, const uint4* buf, int ks) {
+    // One stage: the products of fragment set `slot`, and between them, in the first three quarters, the other set's fragments
+    // are read from buffer `buf` (the last quarter is the time they have to arrive) and, evenly spaced -- the address unit
+    // takes 16 cycles for a piece, and all four waves ask at once --, the pieces of the next asked stage go out: the
+    // matrix unit works on meanwhile.
+    auto stage = [&](auto slot_c, auto last_c, const uint4* buf) {
       constexpr int slot = decltype(slot_c)::value;
       constexpr bool last = decltype(last_c)::value;       // products only
-      constexpr bool more = slot == 1 && !last;
-      unsigned k0 = 0, ow = 0, ox = 0;
-      if constexpr (more) { k0 = ask_k0(); ow = ask_in_k() ? vw : kBufOob; ox = ask_in_k() ? vx : kBufOob; }
+      const unsigned k0 = ask_k0(), ow = ask_in_k() ? vw : kBufOob, ox = ask_in_k() ? vx : kBufOob;
       static_for<NP>([&](auto qc) {
         constexpr int q = decltype(qc)::value, i = q / TW, j = q % TW;
-        acc[i][j] = mfma_32x32x32_i8(wf[slot][i], xf[slot][j], acc[i][j]);
-        sched_fence();
-        constexpr int r0 = 2 * q * NR / NP < NR ? 2 * q * NR / NP : NR, r1 = 2 * (q + 1) * NR / NP < NR ? 2 * (q + 1) * NR / NP : NR;
+        if constexpr (BIG) mfma_16x16x64_i8_agpr(acc[i][j], wf[slot][i], xf[slot][j]);
+        else acc[i][j] = mfma_16x16x64_i8(wf[slot][i], xf[slot][j], acc[i][j]);
         if constexpr (!last) {
+          constexpr int r0 = 4 * q * NR / (3 * NP) < NR ? 4 * q * NR / (3 * NP) : NR;
+          constexpr int r1 = 4 * (q + 1) * NR / (3 * NP) < NR ? 4 * (q + 1) * NR / (3 * NP) : NR;
+          constexpr int p0 = q * 2 * PW / NP, p1 = (q + 1) * 2 * PW / NP;
+          if constexpr (r1 > r0 || p1 > p0) sched_fence();
 #pragma unroll
-          for (int r = r0; r < r1; ++r) read_frag(slot ^ 1, buf, ks, r);
-        }
-        if constexpr (more) {
-          constexpr int h = NP / 2, n = NP - h;
-          constexpr int p0 = q < h ? 0 : (q - h) * 2 * PW / n, p1 = q < h ? 0 : (q + 1 - h) * 2 * PW / n;
+          for (int r = r0; r < r1; ++r) read_frag(slot ^ 1, buf, r);
 #pragma unroll
-          for (int p = p0; p < p1; ++p) ask_piece(p, k0, ow, ox);
+          for (int p = p0; p < p1; ++p) ask_piece(p, k0, p < PW ? ow : ox);
+          if constexpr (r1 > r0 || p1 > p0) sched_fence();
         }
-        sched_fence();
       });
-      if constexpr (more) ask_next();
+      if constexpr (!last) ask_next();
     };
     constexpr std::integral_constant<int, 0> c0{};
     constexpr std::integral_constant<int, 1> c1{};
     constexpr std::false_type no{};
     constexpr std::true_type yes{};
 
+    if constexpr (BIG) agpr_sums_settled();
     describe();
-    for (int q = 0; q < NBUF; ++q) ask_stage();      // (every buffer is empty)
+    for (int q = 0; q < NBUF; ++q) {                 // (every buffer is empty)
+      const unsigned k0 = ask_k0(), ow = ask_in_k() ? vw : kBufOob, ox = ask_in_k() ? vx : kBufOob;
+#pragma unroll
+      for (int p = 0; p < 2 * PW; ++p) ask_piece(p, k0, p < PW ? ow : ox);
+      ask_next();
+    }
     wait_dma_all_but<(NBUF - 1) * 2 * PW>();
     wg_barrier_nodrain();
 #pragma unroll
-    for (int r = 0; r < NR; ++r) read_frag(0, lds, 0, r);
-    int g = 0;                          // stages taken; asked = g + NBUF up to the middle of a stage
+    for (int r = 0; r < NR; ++r) read_frag(0, lds, r);
+    int g = 0;                          // stages taken
+    // behind it: every wave has its fragments of stage g, and stage g + 1 -- of g + 1 .. g + NBUF - 1 in flight -- has landed
+    // (stores and parameter pieces among the newer operations only make the wait stricter)
+    auto turn = [&]() {
+      wait_lds_reads();
+      wait_dma_all_but<(NBUF - 2) * 2 * PW>();
+      wg_barrier_nodrain();
+      ++g;
+    };
     for (int tile = 0;; ++tile) {
-      for (int s = 0; s < cur.ns - (BIG ? 1 : 0); ++s, ++g) {
-        half_stage(c0, no, lds + (g % NBUF) * STAGE, 1);
-        wait_lds_reads();               // this wave's fragments of stage g are in registers
-        // stage g + 1 has landed (stores and parameter pieces among the newer operations only make the wait stricter)
-        wait_dma_all_but<(NBUF - 2) * 2 * PW>();
-        wg_barrier_nodrain();
-        half_stage(c1, no, lds + ((g + 1) % NBUF) * STAGE, 0);  // asks into the buffer that stage g leaves
-      }
-      if constexpr (BIG) {              // (the sums leave their accumulators from the block that finishes them)
-        half_stage(c0, no, lds + (g % NBUF) * STAGE, 1);
-        half_stage(c1, yes, lds, 0);
+      for (int s = 0; s < cur.ns; s += 2) {
+        turn();
+        stage(c0, no, lds + (g % NBUF) * STAGE);
+        turn();
+        stage(c1, no, lds + (g % NBUF) * STAGE);
       }
       finish(cur, params + (tile % 3) * SLOT);
-      if constexpr (BIG) break;
+      if constexpr (BIG) break;         // (one tile a workgroup)
       id += gx;
       if (id >= xend) break;
       cur = item_of(id);
@@ -476,6 +477,7 @@ __global__ __launch_bounds__(256, B > 128 ? 1 : 3) void i8_tile_kernel(const I8A
     constexpr int CH = STAGE / 256;       // chunks of a thread per stage
     constexpr int AHEAD = B > 64 ? 2 : 4;   // stages in registers
     uint4 q[AHEAD][CH];
+    const int ns = cur.s_end - cur.s_begin;
     auto fetch = [&](int s, uint4 (&to)[CH]) {
       const int k0 = (cur.s_begin + s) * 64;
 #pragma unroll
@@ -486,31 +488,28 @@ __global__ __launch_bounds__(256, B > 128 ? 1 : 3) void i8_tile_kernel(const I8A
         else if (cur.m0 + row - B < a.m) to[p] = i8_chunk(a.x + (cur.m0 + row - B) * a.ldx, at, a.k);
       }
     };
-    static_for<AHEAD>([&](auto d) { if (decltype(d)::value < cur.ns) fetch(decltype(d)::value, q[decltype(d)::value]); });
-    for (int s0 = 0; s0 < cur.ns; s0 += AHEAD)
+    static_for<AHEAD>([&](auto d) { if (decltype(d)::value < ns) fetch(decltype(d)::value, q[decltype(d)::value]); });
+    for (int s0 = 0; s0 < ns; s0 += AHEAD)
       static_for<AHEAD>([&](auto d) {
         constexpr int v = decltype(d)::value;
         const int s = s0 + v;
-        if (s < cur.ns) {
+        if (s < ns) {
           uint4* const buf = lds + (s & 1) * STAGE;
 #pragma unroll
           for (int p = 0; p < CH; ++p) {
             const int id4 = p * 256 + tid, row = id4 >> 2;
-            buf[row * 4 + ((id4 & 3) ^ ((row >> 2) & 3))] = q[v][p];
+            buf[row * 4 + ((id4 & 3) ^ (-(row >> 2) & 3))] = q[v][p];
           }
-          if (s + AHEAD < cur.ns) fetch(s + AHEAD, q[v]);
+          if (s + AHEAD < ns) fetch(s + AHEAD, q[v]);
           // (one barrier a stage: a wave may write buffer s+1 -- last read in stage s-1 -- while others still read buffer s)
           wait_lds_reads();
           wg_barrier_nodrain();
 #pragma unroll
-          for (int ks = 0; ks < 2; ++ks) {
+          for (int r = 0; r < NR; ++r) read_frag(0, buf, r);
 #pragma unroll
-            for (int r = 0; r < NR; ++r) read_frag(0, buf, ks, r);
+          for (int i = 0; i < TW; ++i)
 #pragma unroll
-            for (int i = 0; i < TW; ++i)
-#pragma unroll
-              for (int j = 0; j < TW; ++j) acc[i][j] = mfma_32x32x32_i8(wf[0][i], xf[0][j], acc[i][j]);
-          }
+            for (int j = 0; j < TW; ++j) acc[i][j] = mfma_16x16x64_i8(wf[0][i], xf[0][j], acc[i][j]);
         }
       });
     finish(cur, params);

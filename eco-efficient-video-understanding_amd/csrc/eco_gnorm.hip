@@ -1,13 +1,19 @@
 // eco_gnorm.hip -- group norm with an activation over channels-last positions (include/eco_hip.h, ABI v20).
 //
 //   y = act((x - mean) / sqrt(var + eps) * gamma + beta),  mean / var over an image's valid positions x c/groups channels
+//
+// Bound by memory: x has to be read once and y written once, ten operations a value.  Two forms:
+//   slab   groups of an image whose values fit the registers of one workgroup: read once, mean, squared differences from it
+//          and result from registers, written once; one launch
+//   split  larger images: one launch reads x and leaves (mean, sum of squared differences) of every group's part in a chunk of
+//          positions, a second joins the parts and reads x again -- from the last-level cache where x fits it
+// All sums are fp32.  Squared differences are always taken from a mean of the values at hand, never as a difference of large sums:
+//   parts (n_i, m_i, q_i) join as  m = m_0 + sum n_i (m_i - m_0) / n,  q = sum q_i + n_i (m_i - m)^2.
 #include <math.h>
 
 #include "eco_common.h"
 
 namespace eco {
-
-constexpr int kGnThreads = 256;
 
 struct GnArgs {
   const void* x;
@@ -15,68 +21,518 @@ struct GnArgs {
   const int* lengths;
   const float* gamma;
   const float* beta;
+  float2* part;                          // split: [n][chunks][groups + tiles - 1] (mean, sum of squared differences)
   long x_image, x_row, y_image, y_row;   // strides in elements
-  long s;
+  long s, n;
   int c, groups, cg;
   int act;
   float eps;
+  int cv;                                // vectors of a row that a workgroup takes (slab: of its groups, split: of its channel tile)
+  int rows_par;                          // rows that its threads take at once
+  int gb, slabs;                         // slab: groups of a workgroup, workgroups of an image
+  int chunks, rows_chunk, tiles;         // split
 };
 
-template <typename T>
-__device__ __forceinline__ float gn_load(const T* p);
+// VEC consecutive values of a row as one load: 16 bytes where the pointers and strides allow it, 4 bytes or one value otherwise
+template <typename T, int VEC>
+struct GnVec;
 template <>
-__device__ __forceinline__ float gn_load<float>(const float* p) { return ld(p); }
+struct GnVec<float, 4> {
+  typedef uint4 raw;
+  // (unpacked once more where it is used once more: the values of a batch do not fit the registers)
+  static __device__ __forceinline__ void again(raw& r) { ECO_OPAQUE(r.x); ECO_OPAQUE(r.y); ECO_OPAQUE(r.z); ECO_OPAQUE(r.w); }
+  static __device__ __forceinline__ void get(const raw& r, float (&v)[4]) {
+    __builtin_memcpy(v, &r, 16);
+  }
+  static __device__ __forceinline__ raw put(const float (&v)[4]) {
+    raw r;
+    __builtin_memcpy(&r, v, 16);
+    return r;
+  }
+};
 template <>
-__device__ __forceinline__ float gn_load<unsigned short>(const unsigned short* p) { return bf16_bits_to_f32(ld(p)); }
-__device__ __forceinline__ void gn_store(float* p, float v) { st(p, v); }
-__device__ __forceinline__ void gn_store(unsigned short* p, float v) { st(p, (unsigned short)f32_to_bf16_bits(v)); }
+struct GnVec<float, 1> {
+  typedef float raw;
+  static __device__ __forceinline__ void again(raw&) {}
+  static __device__ __forceinline__ void get(const raw& r, float (&v)[1]) { v[0] = r; }
+  static __device__ __forceinline__ raw put(const float (&v)[1]) { return v[0]; }
+};
+template <>
+struct GnVec<unsigned short, 8> {
+  typedef uint4 raw;
+  // (unpacked once more where it is used once more: the values of a batch do not fit the registers)
+  static __device__ __forceinline__ void again(raw& r) { ECO_OPAQUE(r.x); ECO_OPAQUE(r.y); ECO_OPAQUE(r.z); ECO_OPAQUE(r.w); }
+  static __device__ __forceinline__ void get(const raw& r, float (&v)[8]) {
+    const unsigned w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] = bf16_bits_to_f32(w[i] & 0xffffu);
+      v[2 * i + 1] = bf16_bits_to_f32(w[i] >> 16);
+    }
+  }
+  static __device__ __forceinline__ raw put(const float (&v)[8]) {
+    return make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+  }
+};
+template <>
+struct GnVec<unsigned short, 2> {
+  typedef unsigned raw;
+  static __device__ __forceinline__ void again(raw&) {}
+  static __device__ __forceinline__ void get(const raw& r, float (&v)[2]) {
+    v[0] = bf16_bits_to_f32(r & 0xffffu);
+    v[1] = bf16_bits_to_f32(r >> 16);
+  }
+  static __device__ __forceinline__ raw put(const float (&v)[2]) { return pack_bf16x2(v[0], v[1]); }
+};
+template <>
+struct GnVec<unsigned short, 1> {
+  typedef unsigned short raw;
+  static __device__ __forceinline__ void again(raw&) {}
+  static __device__ __forceinline__ void get(const raw& r, float (&v)[1]) { v[0] = bf16_bits_to_f32(r); }
+  static __device__ __forceinline__ raw put(const float (&v)[1]) { return (unsigned short)f32_to_bf16_bits(v[0]); }
+};
 
-__device__ __forceinline__ float gn_act(float v, int act) {
-  if (act == ECO_ACT_RELU) return v < 0.0f ? 0.0f : v;      // (a NaN stays)
-  if (act == ECO_ACT_SILU) return silu(v);
+__device__ __forceinline__ long gn_rows(const GnArgs& a, long img) {
+  if (!a.lengths) return a.s;
+  const long len = ld(a.lengths + img);
+  return len < 0 ? 0 : len > a.s ? a.s : len;
+}
+
+template <int VEC>
+__device__ __forceinline__ void gn_activate(float (&v)[VEC], int act) {
+  if (act == ECO_ACT_RELU) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v[e] = v[e] < 0.0f ? 0.0f : v[e];      // (a NaN stays)
+  } else if (act == ECO_ACT_SILU) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v[e] = silu(v[e]);
+  }
+}
+
+// Lanes that sum one group's entries: a power of two, so that all of `groups` are summed at once where threads suffice.
+__device__ __forceinline__ int gn_lanes(int threads, int groups) {
+  int l = kWave;
+  while (l > 1 && l * groups > threads) l >>= 1;
+  return l;
+}
+// Sum over the aligned `lanes` lanes of a wave; every lane of them gets it.  (Called by whole waves.)
+__device__ __forceinline__ float gn_lane_sum(float v, int lanes) {
+  for (int m = lanes >> 1; m >= 1; m >>= 1) v += shfl_xor(v, m);
   return v;
 }
 
-// Sum over the workgroup, every thread gets it; the order is fixed.
-__device__ __forceinline__ float gn_block_sum(float v, float* red) {
-  v = wave_sum(v);
-  if (lane_id() == 0) red[threadIdx.x >> 6] = v;
-  __syncthreads();
-  const float t = (red[0] + red[1]) + (red[2] + red[3]);
-  __syncthreads();
-  return t;
+// e / per for 0 <= e < 2^16, inv = fp32(1 / per): e + 1/2 is no nearer to a multiple of per than 1/2, a relative distance of 2^-17.
+__device__ __forceinline__ int gn_div(int e, float inv) { return (int)(((float)e + 0.5f) * inv); }
+
+// ---- slab ------------------------------------------------------------------------------------------------------------------------
+// Entries [rows][units] in LDS (a unit: a vector where vectors lie inside groups, else a channel) -> one sum per group of
+// `per` units, left in out[]; f turns (sum) into what is stored.
+template <typename F>
+__device__ __forceinline__ void gn_group_sums(const float* red, int rows, int units, int per, int groups, float* out, F f) {
+  const int threads = (int)blockDim.x, lanes = gn_lanes(threads, groups);
+  const int j = (int)threadIdx.x & (lanes - 1);
+  const float inv = 1.0f / (float)per;
+  for (int g0 = 0; g0 < groups; g0 += threads / lanes) {
+    const int g = g0 + (int)threadIdx.x / lanes;
+    float sum = 0.0f;
+    if (g < groups) {
+#pragma unroll 4
+      for (int e = j; e < rows * per; e += lanes) {
+        const int r = gn_div(e, inv);
+        sum += red[r * units + g * per + (e - r * per)];
+      }
+    }
+    sum = gn_lane_sum(sum, lanes);
+    if (j == 0 && g < groups) out[g] = f(sum);
+  }
 }
 
-// One workgroup per (image, group): mean, then the sum of squared differences, then the result, each a pass over the
-// group's values.
-template <typename T>
-__global__ __launch_bounds__(256) void group_norm_kernel(const GnArgs a) {
-  __shared__ float red[4];
-  const int g = (int)(blockIdx.x % (unsigned)a.groups);
-  const long img = (long)(blockIdx.x / (unsigned)a.groups);
-  long rows = a.s;
-  if (a.lengths) {
-    const long len = ld(a.lengths + img);
-    rows = len < 0 ? 0 : len > a.s ? a.s : len;
+// Registers of a slab's thread: R vectors, three floats a channel and as much again for the work -- as waves a SIMD that leaves.
+constexpr int gn_slab_waves(int r, int bytes) { return bytes == 16 ? (r > 8 ? 4 : r > 2 ? 6 : 8) : (r > 32 ? 4 : 8); }
+
+// One workgroup per (image, gb groups); thread (rp, col) holds rows rp, rp + rows_par, ... of one vector of channels in registers.
+// Slabs of an image are neighbours on an XCD: their rows share cache lines.
+template <typename T, int VEC, int R>
+__global__ __launch_bounds__(512, gn_slab_waves(R, VEC * (int)sizeof(T))) void gn_slab_kernel(const GnArgs a) {
+  typedef GnVec<T, VEC> V;
+  ECO_DYNAMIC_LDS(red);                                     // [blockDim][VEC], then mean and 1 / spread of each group
+  const int threads = (int)blockDim.x, tid = (int)threadIdx.x;
+  float* const mean = red + threads * VEC;
+  float* const rstd = mean + a.gb;
+  const unsigned id = (unsigned)xcd_remap((int)blockIdx.x, (int)gridDim.x);
+  const int slab = (int)(id % (unsigned)a.slabs);
+  const long img = (long)(id / (unsigned)a.slabs);
+  const long rows = gn_rows(a, img);
+  if (rows == 0) return;
+  const int g0 = slab * a.gb, groups = a.groups - g0 < a.gb ? a.groups - g0 : a.gb;
+  const int width = groups * a.cg;                          // channels of this slab (the last one may have fewer)
+  const int rp = tid / a.cv, col = tid - rp * a.cv;
+  const bool on = rp < a.rows_par && col * VEC < width;
+  const int ch = on ? col * VEC : 0;                        // (in the slab; idle threads load the first vector, unused)
+  // thread rows hold `full` positions each, the first `over` of them one more: only step `full` is taken by a part of the threads
+  const int nrows = (int)rows, full = nrows / a.rows_par, over = nrows - full * a.rows_par;
+  const bool tail = on && rp < over;
+  typename V::raw raw[R];
+  {
+    const T* x = (const T*)a.x + img * a.x_image + (long)g0 * a.cg + ch + rp * a.x_row;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      if (i <= full && (i < full ? on : tail)) raw[i] = ld((const typename V::raw*)x);
+      x += a.rows_par * a.x_row;
+    }
   }
-  const T* x = (const T*)a.x + img * a.x_image + (long)g * a.cg;
-  T* y = (T*)a.y + img * a.y_image + (long)g * a.cg;
-  const long count = rows * a.cg;
-  float sum = 0.0f;
-  for (long i = threadIdx.x; i < count; i += kGnThreads) sum += gn_load(x + (i / a.cg) * a.x_row + i % a.cg);
-  const float mean = gn_block_sum(sum, red) / (float)count;
-  float sq = 0.0f;
-  for (long i = threadIdx.x; i < count; i += kGnThreads) {
-    const float d = gn_load(x + (i / a.cg) * a.x_row + i % a.cg) - mean;
-    sq += d * d;
+  const bool whole = a.cg % VEC == 0;
+  const int per = whole ? a.cg / VEC : a.cg, units = whole ? a.cv : a.cv * VEC;
+  // a thread's sums into LDS; where a row's vectors are a power of two below a wave, the wave's rows are summed first
+  const bool fold = a.cv < kWave && (a.cv & (a.cv - 1)) == 0;
+  const int red_rows = fold ? threads / kWave : a.rows_par;
+  auto publish = [&](float (&p)[VEC]) {
+    if (whole) {
+#pragma unroll
+      for (int e = 1; e < VEC; ++e) p[0] += p[e];
+    }
+    const int at = fold ? tid >> 6 : rp;
+    if (fold) {
+      for (int m = a.cv; m < kWave; m <<= 1) {
+        p[0] += shfl_xor(p[0], m);
+        if (!whole) {
+#pragma unroll
+          for (int e = 1; e < VEC; ++e) p[e] += shfl_xor(p[e], m);
+        }
+      }
+    }
+    if (fold ? lane_id() < a.cv : rp < a.rows_par) {
+      if (whole) red[at * units + col] = p[0];
+      else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) red[at * units + col * VEC + e] = p[e];
+      }
+    }
+    __syncthreads();
+  };
+  const float inv = 1.0f / ((float)rows * (float)a.cg);
+  float p[VEC], m[VEC], v[VEC];
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) p[e] = 0.0f;
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+    if (i <= full && (i < full ? on : tail)) {
+      V::get(raw[i], v);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) p[e] += v[e];
+    }
+  publish(p);
+  gn_group_sums(red, red_rows, units, per, groups, mean, [&](float t) { return t * inv; });
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) {
+    m[e] = mean[(ch + e) / a.cg];
+    p[e] = 0.0f;
   }
-  const float rstd = 1.0f / sqrtf(gn_block_sum(sq, red) / (float)count + a.eps);
-  for (long i = threadIdx.x; i < count; i += kGnThreads) {
-    const int ch = (int)(i % a.cg);
-    const float scale = rstd * (a.gamma ? ld(a.gamma + g * a.cg + ch) : 1.0f);
-    const float v = (gn_load(x + (i / a.cg) * a.x_row + ch) - mean) * scale + (a.beta ? ld(a.beta + g * a.cg + ch) : 0.0f);
-    gn_store(y + (i / a.cg) * a.y_row + ch, gn_act(v, a.act));
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+    if (i <= full && (i < full ? on : tail)) {
+      V::get(raw[i], v);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) p[e] += (v[e] - m[e]) * (v[e] - m[e]);
+    }
+  publish(p);
+  gn_group_sums(red, red_rows, units, per, groups, rstd, [&](float t) { return 1.0f / sqrtf(t * inv + a.eps); });
+  __syncthreads();
+  float sc[VEC], sh[VEC];
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) {
+    const int at = g0 * a.cg + ch + e;
+    sc[e] = rstd[(ch + e) / a.cg] * (a.gamma ? ld(a.gamma + at) : 1.0f);
+    sh[e] = a.beta ? ld(a.beta + at) : 0.0f;
   }
+  T* y = (T*)a.y + img * a.y_image + (long)g0 * a.cg + ch + rp * a.y_row;
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    if (i <= full && (i < full ? on : tail)) {
+      V::get(raw[i], v);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) v[e] = (v[e] - m[e]) * sc[e] + sh[e];
+      gn_activate(v, a.act);
+      st((typename V::raw*)y, V::put(v));
+    }
+    y += a.rows_par * a.y_row;
+  }
+}
+
+// ---- split -----------------------------------------------------------------------------------------------------------------------
+// Channel tiles of cv vectors x chunks of rows_chunk positions.  Group g's part of tile t stands at place g + t of a chunk's
+// row of parts: neighbouring tiles share at most one group, so no two parts meet.
+constexpr int kGnThreads = 256, kGnBatch = 8;
+
+struct GnPlace {
+  long img;
+  int chunk, tile;
+  int ch0, ch1;      // channels of the tile
+  int g0, groups;    // groups that it touches
+};
+template <int VEC>
+__device__ __forceinline__ GnPlace gn_place(const GnArgs& a, int chunks) {
+  GnPlace p;
+  unsigned b = blockIdx.x;
+  p.tile = (int)(b % (unsigned)a.tiles); b /= (unsigned)a.tiles;
+  p.chunk = (int)(b % (unsigned)chunks);
+  p.img = (long)(b / (unsigned)chunks);
+  p.ch0 = p.tile * a.cv * VEC;
+  p.ch1 = p.ch0 + a.cv * VEC < a.c ? p.ch0 + a.cv * VEC : a.c;
+  p.g0 = p.ch0 / a.cg;
+  p.groups = (p.ch1 - 1) / a.cg - p.g0 + 1;
+  return p;
+}
+
+// Statistics: every thread takes one vector of channels over every rows_par-th position of the chunk, eight at a time;
+// differences are summed from the mean of its first eight, so that the squares cannot cancel.
+template <typename T, int VEC>
+__global__ __launch_bounds__(256, 6) void gn_stats_kernel(const GnArgs a) {
+  typedef GnVec<T, VEC> V;
+  __shared__ float lm[kGnThreads * VEC], lq[kGnThreads * VEC];
+  const GnPlace p = gn_place<VEC>(a, a.chunks);
+  const long rows = gn_rows(a, p.img);
+  const long r0 = (long)p.chunk * a.rows_chunk, r1 = r0 + a.rows_chunk < rows ? r0 + a.rows_chunk : rows;
+  if (r0 >= r1) return;
+  const int tid = (int)threadIdx.x, rp = tid / a.cv, col = tid - rp * a.cv;
+  const int ch = p.ch0 + col * VEC;
+  const bool on = rp < a.rows_par && ch < a.c;
+  // thread rows hold each_has positions of the chunk, the first `over` of them one more
+  const int nrows = (int)(r1 - r0), each_has = nrows / a.rows_par, over = nrows - each_has * a.rows_par;
+  const bool tail = on && rp < over;
+  const T* x = (const T*)a.x + p.img * a.x_image + ch + (r0 + rp) * a.x_row;
+  const long step = a.rows_par * a.x_row;
+  float piv[VEC], s1[VEC], s2[VEC];
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) piv[e] = s1[e] = s2[e] = 0.0f;
+  for (int i0 = 0; i0 < each_has + (over ? 1 : 0); i0 += kGnBatch) {
+    typename V::raw raw[kGnBatch];
+#pragma unroll
+    for (int i = 0; i < kGnBatch; ++i) {
+      if (i0 + i <= each_has && (i0 + i < each_has ? on : tail)) raw[i] = ld((const typename V::raw*)x);
+      x += step;
+    }
+    if (i0 == 0) {
+#pragma unroll
+      for (int i = 0; i < kGnBatch; ++i)
+        if (i <= each_has && (i < each_has ? on : tail)) {
+          float v[VEC];
+          V::get(raw[i], v);
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) piv[e] += v[e];
+        }
+      const int has = each_has + (tail ? 1 : 0);
+      const float inv = 1.0f / (float)(has < kGnBatch ? (has > 0 ? has : 1) : kGnBatch);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) piv[e] *= inv;
+    }
+#pragma unroll
+    for (int i = 0; i < kGnBatch; ++i)
+      if (i0 + i <= each_has && (i0 + i < each_has ? on : tail)) {
+        float v[VEC];
+        V::again(raw[i]);
+        V::get(raw[i], v);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          const float d = v[e] - piv[e];
+          s1[e] += d;
+          s2[e] += d * d;
+        }
+      }
+  }
+  auto count = [&](int k) { return (float)(each_has + (k < over ? 1 : 0)); };     // positions of thread row k
+  {
+    const float n = count(rp), inv = n > 0.0f ? 1.0f / n : 0.0f;
+    if (rp < a.rows_par) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const float q = s2[e] - s1[e] * s1[e] * inv;
+        lm[(rp * a.cv + col) * VEC + e] = piv[e] + s1[e] * inv;
+        lq[(rp * a.cv + col) * VEC + e] = q < 0.0f ? 0.0f : q;     // (a NaN stays)
+      }
+    }
+  }
+  __syncthreads();
+  const int lanes = gn_lanes(kGnThreads, p.groups), j = tid & (lanes - 1), width = a.cv * VEC;
+  const int thread_rows = r1 - r0 < a.rows_par ? (int)(r1 - r0) : a.rows_par;     // thread rows that have a position
+  for (int gl = 0; gl < p.groups; gl += kGnThreads / lanes) {
+    const int g = gl + tid / lanes;
+    int from = (p.g0 + g) * a.cg - p.ch0, to = from + a.cg;     // the group's channels in the tile
+    if (from < 0) from = 0;
+    if (to > p.ch1 - p.ch0) to = p.ch1 - p.ch0;
+    const int per = to - from;
+    const bool mine = g < p.groups;
+    const float m0 = mine ? lm[from] : 0.0f;
+    float t = 0.0f;
+    const float ipr = 1.0f / (float)(per > 0 ? per : 1);
+    auto each = [&](auto f) {
+      if (!mine) return;
+#pragma unroll 4
+      for (int e = j; e < thread_rows * per; e += lanes) {
+        const int k = gn_div(e, ipr);
+        f(count(k), k * width + from + (e - k * per));
+      }
+    };
+    each([&](float n, int at) { t += n * (lm[at] - m0); });
+    t = gn_lane_sum(t, lanes);
+    const float m = m0 + t / ((float)(r1 - r0) * (float)(per > 0 ? per : 1));
+    float q = 0.0f;
+    each([&](float n, int at) { q += lq[at] + n * (lm[at] - m) * (lm[at] - m); });
+    q = gn_lane_sum(q, lanes);
+    if (mine && j == 0)
+      st(a.part + ((p.img * a.chunks + p.chunk) * (long)(a.groups + a.tiles - 1) + p.g0 + g + p.tile), make_float2(m, q));
+  }
+}
+
+// Result: joins the parts of its tile's groups, then a pass over its positions.  Images in falling order: what the statistics read
+// last is still in the last-level cache.
+template <typename T, int VEC>
+__global__ __launch_bounds__(256) void gn_apply_kernel(const GnArgs a, int chunks, int rows_chunk) {
+  typedef GnVec<T, VEC> V;
+  __shared__ float mean[kGnThreads * VEC], rstd[kGnThreads * VEC];
+  GnPlace p = gn_place<VEC>(a, chunks);
+  p.img = a.n - 1 - p.img;
+  const long rows = gn_rows(a, p.img);
+  const long r0 = (long)p.chunk * rows_chunk, r1 = r0 + rows_chunk < rows ? r0 + rows_chunk : rows;
+  if (r0 >= r1) return;
+  const int tid = (int)threadIdx.x, rp = tid / a.cv, col = tid - rp * a.cv;
+  const int ch = p.ch0 + col * VEC;
+  const bool on = rp < a.rows_par && ch < a.c;
+  const int lanes = gn_lanes(kGnThreads, p.groups), j = tid & (lanes - 1);
+  const int slots = a.groups + a.tiles - 1;
+  for (int gl = 0; gl < p.groups; gl += kGnThreads / lanes) {
+    const int g = gl + tid / lanes;
+    const bool mine = g < p.groups;
+    const int c0 = (p.g0 + (mine ? g : 0)) * a.cg, t0 = c0 / (a.cv * VEC), t1 = (c0 + a.cg - 1) / (a.cv * VEC);
+    const float2* const part = a.part + p.img * a.chunks * (long)slots + p.g0 + g;
+    const float m0 = mine ? ld(&part[t0]).x : 0.0f;
+    auto each = [&](auto f) {
+      if (!mine) return;
+      for (int t = t0; t <= t1; ++t) {
+        const int lo = c0 > t * a.cv * VEC ? c0 : t * a.cv * VEC;
+        const int hi = c0 + a.cg < (t + 1) * a.cv * VEC ? c0 + a.cg : (t + 1) * a.cv * VEC;
+        for (int k = j; k < a.chunks; k += lanes) {
+          long in = rows - (long)k * a.rows_chunk;
+          if (in <= 0) break;                                     // (a chunk behind the image's length left no part)
+          in = in < a.rows_chunk ? in : a.rows_chunk;
+          f((float)in * (float)(hi - lo), ld(part + (long)k * slots + t));
+        }
+      }
+    };
+    float t = 0.0f, q = 0.0f;
+    each([&](float n, float2 v) { t += n * (v.x - m0); });
+    t = gn_lane_sum(t, lanes);
+    const float total = (float)rows * (float)a.cg, m = m0 + t / total;
+    each([&](float n, float2 v) { q += v.y + n * (v.x - m) * (v.x - m); });
+    q = gn_lane_sum(q, lanes);
+    if (mine && j == 0) {
+      mean[g] = m;
+      rstd[g] = 1.0f / sqrtf(q / total + a.eps);
+    }
+  }
+  __syncthreads();
+  if (!on) return;
+  float m[VEC], sc[VEC], sh[VEC];
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) {
+    const int g = (ch + e) / a.cg - p.g0;
+    m[e] = mean[g];
+    sc[e] = rstd[g] * (a.gamma ? ld(a.gamma + ch + e) : 1.0f);
+    sh[e] = a.beta ? ld(a.beta + ch + e) : 0.0f;
+  }
+  const T* const x = (const T*)a.x + p.img * a.x_image + ch;
+  T* const y = (T*)a.y + p.img * a.y_image + ch;
+  constexpr int U = 4;
+  for (long r = r0 + rp; r < r1; r += (long)U * a.rows_par) {
+    typename V::raw raw[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const long row = r + (long)i * a.rows_par;
+      raw[i] = ld((const typename V::raw*)(x + (row < r1 ? row : r) * a.x_row));
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const long row = r + (long)i * a.rows_par;
+      if (row < r1) {
+        float v[VEC];
+        V::get(raw[i], v);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[e] = (v[e] - m[e]) * sc[e] + sh[e];
+        gn_activate(v, a.act);
+        st((typename V::raw*)(y + row * a.y_row), V::put(v));
+      }
+    }
+  }
+}
+
+// ---- host ------------------------------------------------------------------------------------------------------------------------
+constexpr int kGnSlabThreads = 512;
+constexpr int kGnMaxChunks = 256;        // every result workgroup reads the parts of all chunks of its image
+
+// Vectors that a thread of a slab holds at most: 64 registers, so that two workgroups of 512 threads share a compute unit and one
+// loads or stores while the other sums.
+constexpr int gn_held(int vec, int es) { return vec * es == 16 ? 16 : 64; }
+
+struct GnSlab {
+  int gb, cv;
+};
+// Groups of a slab: the fewest that give rows of 64 bytes and whole vectors, or the most that fit where those do not.
+static bool gn_slab_fits(long s, int cg, int groups, int vec, int es, GnSlab* out) {
+  bool found = false;
+  for (int gb = 1; gb <= groups; ++gb) {
+    const long width = (long)gb * cg;
+    if (width % vec) continue;
+    const long cv = width / vec;
+    if (cv > kGnSlabThreads || ceil_div(s, kGnSlabThreads / cv) > gn_held(vec, es)) break;
+    out->gb = gb; out->cv = (int)cv;
+    found = true;
+    if (width * es >= 64) break;
+  }
+  return found;
+}
+
+template <typename T, int VEC>
+static int gn_launch(const eco_group_norm_plan& p, GnArgs& a, hipStream_t st) {
+  GnSlab sl;
+  if (gn_slab_fits(p.s, a.cg, p.groups, VEC, (int)sizeof(T), &sl)) {
+    a.gb = sl.gb; a.cv = sl.cv; a.slabs = (int)ceil_div(p.groups, sl.gb);
+    // threads: the most, or -- where the launch fills the device anyway, or the rows are fewer -- no more than the values need
+    constexpr int R = gn_held(VEC, (int)sizeof(T));
+    long threads = kGnSlabThreads;
+    while (threads > 256 && threads / 2 >= sl.cv && ceil_div(p.s, threads / 2 / sl.cv) <= R / 2 &&
+           (p.n * a.slabs >= 4l * p.num_cu || threads / 2 >= sl.cv * p.s))
+      threads /= 2;
+    a.rows_par = (int)(threads / sl.cv);
+    const long held = ceil_div(p.s, a.rows_par);          // vectors a thread
+    const dim3 grid((unsigned)(p.n * a.slabs)), block((unsigned)threads);
+    const unsigned lds = (unsigned)((threads * VEC + 2 * sl.gb) * 4);
+    if (held <= R / 8) hipLaunchKernelGGL((gn_slab_kernel<T, VEC, R / 8>), grid, block, lds, st, a);
+    else if (held <= R / 2) hipLaunchKernelGGL((gn_slab_kernel<T, VEC, R / 2>), grid, block, lds, st, a);
+    else hipLaunchKernelGGL((gn_slab_kernel<T, VEC, R>), grid, block, lds, st, a);
+    return check_launch("eco_group_norm_forward");
+  }
+  const long vecs = ceil_div(p.c, VEC);
+  a.tiles = (int)ceil_div(vecs, kGnThreads);
+  a.cv = (int)ceil_div(vecs, a.tiles);
+  a.tiles = (int)ceil_div(vecs, a.cv);
+  a.rows_par = kGnThreads / a.cv;
+  // (chunks of whole batches, so no more of them than the plan's)
+  a.rows_chunk = (int)(ceil_div(ceil_div(p.s, p.chunks), kGnBatch * a.rows_par) * kGnBatch * a.rows_par);
+  a.chunks = (int)ceil_div(p.s, a.rows_chunk);
+  const long parts = p.n * a.chunks * a.tiles;
+  // result: eight workgroups a compute unit, of four rows a thread at least
+  long chunks = ceil_div(8l * p.num_cu, p.n * a.tiles);
+  const long most = ceil_div(p.s, 4l * a.rows_par);
+  if (chunks > most) chunks = most;
+  const int rows_chunk = (int)ceil_div(p.s, chunks);
+  chunks = ceil_div(p.s, rows_chunk);
+  const long results = p.n * chunks * a.tiles;
+  ECO_REQUIRE(parts <= 2147483647l && results <= 2147483647l, "group_norm: too many positions, images and channels for one launch");
+  hipLaunchKernelGGL((gn_stats_kernel<T, VEC>), dim3((unsigned)parts), dim3(kGnThreads), 0, st, a);
+  if (int rc = check_launch("eco_group_norm_forward(statistics)")) return rc;
+  hipLaunchKernelGGL((gn_apply_kernel<T, VEC>), dim3((unsigned)results), dim3(kGnThreads), 0, st, a, (int)chunks, rows_chunk);
+  return check_launch("eco_group_norm_forward");
 }
 
 }  // namespace eco
@@ -96,6 +552,22 @@ extern "C" int eco_group_norm_plan_create(int64_t n, int64_t s, int32_t c, int32
   plan->n = n; plan->s = s; plan->c = c; plan->groups = groups; plan->dt = dt;
   plan->num_cu = num_cu ? num_cu : current_device_num_cu();
   plan->chunks = 1;
+  if (n == 0 || s == 0) return ECO_OK;
+  // no workspace where the slab form holds whatever the pointers' alignment turns out to be
+  GnSlab sl;
+  const int es = dt == ECO_DT_F32 ? 4 : 2, cg = c / groups, wide = 16 / es;
+  const bool always = gn_slab_fits(s, cg, groups, 1, es, &sl) && (c % wide || gn_slab_fits(s, cg, groups, wide, es, &sl)) &&
+                      (es == 4 || c % 2 || gn_slab_fits(s, cg, groups, 2, es, &sl));
+  if (always) return ECO_OK;
+  // statistics: eight workgroups a compute unit, of a batch of positions a thread at least
+  const long vecs = c % wide ? c : c / wide, tiles = ceil_div(vecs, kGnThreads);
+  const long rows_par = kGnThreads / ceil_div(vecs, tiles);
+  long chunks = ceil_div(8l * plan->num_cu, n * tiles);
+  const long most = ceil_div(s, kGnBatch * rows_par);
+  if (chunks > most) chunks = most;
+  if (chunks > kGnMaxChunks) chunks = kGnMaxChunks;
+  plan->chunks = (int32_t)chunks;
+  plan->ws_bytes = n * chunks * (groups + ceil_div(c, kGnThreads) - 1) * (int64_t)sizeof(float2);
   return ECO_OK;
 }
 
@@ -115,6 +587,7 @@ extern "C" int eco_group_norm_forward(const eco_group_norm_plan* plan, const voi
   const size_t es = plan->dt == ECO_DT_F32 ? 4 : 2;
   ECO_REQUIRE((uintptr_t)x % es == 0 && (uintptr_t)y % es == 0, "group_norm: x or y is not aligned to its type");
   GnArgs a;
+  memset(&a, 0, sizeof(a));
   a.x = x; a.y = y; a.lengths = lengths; a.gamma = gamma; a.beta = beta;
   a.x_row = x_row_stride ? x_row_stride : plan->c;
   a.y_row = y_row_stride ? y_row_stride : plan->c;
@@ -126,10 +599,17 @@ extern "C" int eco_group_norm_forward(const eco_group_norm_plan* plan, const voi
   ECO_REQUIRE(a.x_image >= 0 && a.y_image >= y_ext, "group_norm: an image stride is too small");
   ECO_REQUIRE(extent_fits(plan->n, a.x_image, x_ext) && extent_fits(plan->n, a.y_image, y_ext), "group_norm: image stride too large");
   ECO_REQUIRE(plan->ws_bytes == 0 || workspace, "group_norm: this plan needs %ld bytes of workspace", (long)plan->ws_bytes);
-  a.s = plan->s; a.c = plan->c; a.groups = plan->groups; a.cg = plan->c / plan->groups; a.act = act; a.eps = eps;
+  ECO_REQUIRE((uintptr_t)workspace % 8 == 0, "group_norm: workspace is not aligned to 8 bytes");
+  a.part = (float2*)workspace;
+  a.s = plan->s; a.n = plan->n; a.c = plan->c; a.groups = plan->groups; a.cg = plan->c / plan->groups; a.act = act; a.eps = eps;
   hipStream_t st = (hipStream_t)stream;
-  const dim3 grid((unsigned)(plan->n * plan->groups)), block(kGnThreads);
-  if (plan->dt == ECO_DT_F32) hipLaunchKernelGGL((group_norm_kernel<float>), grid, block, 0, st, a);
-  else hipLaunchKernelGGL((group_norm_kernel<unsigned short>), grid, block, 0, st, a);
-  return check_launch("eco_group_norm_forward");
+  // vectors: rows and images of both tensors on their boundaries, channels a multiple
+  const auto allowed = [&](int vec) {
+    const size_t b = vec * es;
+    return plan->c % vec == 0 && (uintptr_t)x % b == 0 && (uintptr_t)y % b == 0 && a.x_row % vec == 0 && a.y_row % vec == 0 &&
+           a.x_image % vec == 0 && a.y_image % vec == 0;
+  };
+  if (plan->dt == ECO_DT_F32) return allowed(4) ? gn_launch<float, 4>(*plan, a, st) : gn_launch<float, 1>(*plan, a, st);
+  if (allowed(8)) return gn_launch<unsigned short, 8>(*plan, a, st);
+  return allowed(2) ? gn_launch<unsigned short, 2>(*plan, a, st) : gn_launch<unsigned short, 1>(*plan, a, st);
 }

@@ -288,7 +288,7 @@ __device__ __forceinline__ GnPlace gn_place(const GnArgs& a, int chunks) {
 // Statistics: every thread takes one vector of channels over every rows_par-th position of the chunk, eight at a time;
 // differences are summed from the mean of its first eight, so that the squares cannot cancel.
 template <typename T, int VEC>
-__global__ __launch_bounds__(256, 6) void gn_stats_kernel(const GnArgs a) {
+__global__ __launch_bounds__(256, 5) void gn_stats_kernel(const GnArgs a) {
   typedef GnVec<T, VEC> V;
   __shared__ float lm[kGnThreads * VEC], lq[kGnThreads * VEC];
   const GnPlace p = gn_place<VEC>(a, a.chunks);
@@ -300,46 +300,50 @@ __global__ __launch_bounds__(256, 6) void gn_stats_kernel(const GnArgs a) {
   const bool on = rp < a.rows_par && ch < a.c;
   // thread rows hold each_has positions of the chunk, the first `over` of them one more
   const int nrows = (int)(r1 - r0), each_has = nrows / a.rows_par, over = nrows - each_has * a.rows_par;
-  const bool tail = on && rp < over;
-  const T* x = (const T*)a.x + p.img * a.x_image + ch + (r0 + rp) * a.x_row;
+  // (threads without a vector or a thread row read the first ones again, uncounted: no load is conditional)
+  const int row = rp < a.rows_par && rp < nrows ? rp : 0;
+  const T* const x0 = (const T*)a.x + p.img * a.x_image + (on ? ch : p.ch0) + r0 * a.x_row;
+  const T* x = x0 + row * a.x_row;
   const long step = a.rows_par * a.x_row;
   float piv[VEC], s1[VEC], s2[VEC];
 #pragma unroll
   for (int e = 0; e < VEC; ++e) piv[e] = s1[e] = s2[e] = 0.0f;
-  for (int i0 = 0; i0 < each_has + (over ? 1 : 0); i0 += kGnBatch) {
+  auto batch = [&](int i0, auto whole_c) {
+    constexpr bool whole = decltype(whole_c)::value;       // every thread row has all of the batch's positions
+    const int has = each_has - i0 + (row < over ? 1 : 0);   // (positions behind them: the row's first of the batch, or the chunk's)
     typename V::raw raw[kGnBatch];
 #pragma unroll
-    for (int i = 0; i < kGnBatch; ++i) {
-      if (i0 + i <= each_has && (i0 + i < each_has ? on : tail)) raw[i] = ld((const typename V::raw*)x);
-      x += step;
-    }
+    for (int i = 0; i < kGnBatch; ++i) raw[i] = ld((const typename V::raw*)(x + (whole || i < has ? i * step : 0)));
+    x += kGnBatch * step;
     if (i0 == 0) {
 #pragma unroll
-      for (int i = 0; i < kGnBatch; ++i)
-        if (i <= each_has && (i < each_has ? on : tail)) {
-          float v[VEC];
-          V::get(raw[i], v);
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) piv[e] += v[e];
-        }
-      const int has = each_has + (tail ? 1 : 0);
-      const float inv = 1.0f / (float)(has < kGnBatch ? (has > 0 ? has : 1) : kGnBatch);
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) piv[e] *= inv;
-    }
-#pragma unroll
-    for (int i = 0; i < kGnBatch; ++i)
-      if (i0 + i <= each_has && (i0 + i < each_has ? on : tail)) {
+      for (int i = 0; i < kGnBatch; ++i) {
         float v[VEC];
-        V::again(raw[i]);
         V::get(raw[i], v);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          const float d = v[e] - piv[e];
-          s1[e] += d;
-          s2[e] += d * d;
-        }
+        for (int e = 0; e < VEC; ++e) piv[e] += v[e] * (1.0f / kGnBatch);
       }
+    }
+#pragma unroll
+    for (int i = 0; i < kGnBatch; ++i) {
+      float v[VEC];
+      V::again(raw[i]);
+      V::get(raw[i], v);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        float d = v[e] - piv[e];
+        if (!whole && i >= has) d = 0.0f;
+        s1[e] += d;
+        s2[e] += d * d;
+      }
+    }
+  };
+  int i0 = 0;
+  for (; i0 + kGnBatch <= each_has; i0 += kGnBatch) batch(i0, std::true_type{});
+  if (i0 < each_has + (over ? 1 : 0)) {
+    // (a thread row whose positions are used up: x points behind the chunk)
+    if (i0 >= each_has + (row < over ? 1 : 0)) x = x0;
+    batch(i0, std::false_type{});
   }
   auto count = [&](int k) { return (float)(each_has + (k < over ? 1 : 0)); };     // positions of thread row k
   {
@@ -388,7 +392,7 @@ __global__ __launch_bounds__(256, 6) void gn_stats_kernel(const GnArgs a) {
 // Result: joins the parts of its tile's groups, then a pass over its positions.  Images in falling order: what the statistics read
 // last is still in the last-level cache.
 template <typename T, int VEC>
-__global__ __launch_bounds__(256) void gn_apply_kernel(const GnArgs a, int chunks, int rows_chunk) {
+__global__ __launch_bounds__(256, 6) void gn_apply_kernel(const GnArgs a, int chunks, int rows_chunk) {
   typedef GnVec<T, VEC> V;
   __shared__ float mean[kGnThreads * VEC], rstd[kGnThreads * VEC];
   GnPlace p = gn_place<VEC>(a, chunks);
@@ -441,28 +445,31 @@ __global__ __launch_bounds__(256) void gn_apply_kernel(const GnArgs a, int chunk
     sc[e] = rstd[g] * (a.gamma ? ld(a.gamma + ch + e) : 1.0f);
     sh[e] = a.beta ? ld(a.beta + ch + e) : 0.0f;
   }
-  const T* const x = (const T*)a.x + p.img * a.x_image + ch;
-  T* const y = (T*)a.y + p.img * a.y_image + ch;
-  constexpr int U = 4;
-  for (long r = r0 + rp; r < r1; r += (long)U * a.rows_par) {
+  const int nrows = (int)(r1 - r0), mine = nrows > rp ? (nrows - rp + a.rows_par - 1) / a.rows_par : 0;
+  const T* x = (const T*)a.x + p.img * a.x_image + ch + (r0 + rp) * a.x_row;
+  T* y = (T*)a.y + p.img * a.y_image + ch + (r0 + rp) * a.y_row;
+  const long xstep = a.rows_par * a.x_row, ystep = a.rows_par * a.y_row;
+  auto result = [&](typename V::raw raw, T* to) {
+    float v[VEC];
+    V::get(raw, v);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v[e] = (v[e] - m[e]) * sc[e] + sh[e];
+    gn_activate(v, a.act);
+    st((typename V::raw*)to, V::put(v));
+  };
+  constexpr int U = kGnBatch / 2;
+  int i = 0;
+  for (; i + U <= mine; i += U) {
     typename V::raw raw[U];
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const long row = r + (long)i * a.rows_par;
-      raw[i] = ld((const typename V::raw*)(x + (row < r1 ? row : r) * a.x_row));
-    }
+    for (int u = 0; u < U; ++u) { raw[u] = ld((const typename V::raw*)x); x += xstep; }
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const long row = r + (long)i * a.rows_par;
-      if (row < r1) {
-        float v[VEC];
-        V::get(raw[i], v);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) v[e] = (v[e] - m[e]) * sc[e] + sh[e];
-        gn_activate(v, a.act);
-        st((typename V::raw*)(y + row * a.y_row), V::put(v));
-      }
-    }
+    for (int u = 0; u < U; ++u) { result(raw[u], y); y += ystep; }
+  }
+  for (; i < mine; ++i) {
+    result(ld((const typename V::raw*)x), y);
+    x += xstep;
+    y += ystep;
   }
 }
 
@@ -521,12 +528,10 @@ static int gn_launch(const eco_group_norm_plan& p, GnArgs& a, hipStream_t st) {
   a.rows_chunk = (int)(ceil_div(ceil_div(p.s, p.chunks), kGnBatch * a.rows_par) * kGnBatch * a.rows_par);
   a.chunks = (int)ceil_div(p.s, a.rows_chunk);
   const long parts = p.n * a.chunks * a.tiles;
-  // result: eight workgroups a compute unit, of four rows a thread at least
-  long chunks = ceil_div(8l * p.num_cu, p.n * a.tiles);
-  const long most = ceil_div(p.s, 4l * a.rows_par);
-  if (chunks > most) chunks = most;
-  const int rows_chunk = (int)ceil_div(p.s, chunks);
-  chunks = ceil_div(p.s, rows_chunk);
+  // result: eight workgroups a compute unit, of whole batches of positions
+  const long wanted = ceil_div(8l * p.num_cu, p.n * a.tiles);
+  const int rows_chunk = (int)(ceil_div(ceil_div(p.s, wanted), kGnBatch / 2 * a.rows_par) * kGnBatch / 2 * a.rows_par);
+  const long chunks = ceil_div(p.s, rows_chunk);
   const long results = p.n * chunks * a.tiles;
   ECO_REQUIRE(parts <= 2147483647l && results <= 2147483647l, "group_norm: too many positions, images and channels for one launch");
   hipLaunchKernelGGL((gn_stats_kernel<T, VEC>), dim3((unsigned)parts), dim3(kGnThreads), 0, st, a);

@@ -408,6 +408,21 @@ __device__ __forceinline__ void st(T* p, T v) {
   *p = v;
 }
 
+// Streaming store: a result that this launch does not read again should not push out of the last-level cache what it reads.
+template <typename T>
+__device__ __forceinline__ void st_stream(T* p, T v) {
+#ifdef ECO_EMU
+  st(p, v);
+#else
+  if constexpr (sizeof(T) == 16) {
+    typedef unsigned u32x4_s __attribute__((ext_vector_type(4)));
+    __builtin_nontemporal_store(__builtin_bit_cast(u32x4_s, v), (u32x4_s*)p);
+  } else {
+    __builtin_nontemporal_store(v, p);
+  }
+#endif
+}
+
 // Load from (wave-uniform base) + (per-lane 32-bit byte offset): the `saddr` form of global_load -- SGPR base, VGPR
 // offset, immediate -- so that a stream of loads off one uniform base costs no per-lane 64-bit address arithmetic.
 // (Beside f32 MFMAs every VALU instruction is ~6 cycles of matrix-pipe time: profiles/r03_notes.md.)

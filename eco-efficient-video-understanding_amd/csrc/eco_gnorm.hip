@@ -31,6 +31,7 @@ struct GnArgs {
   int rows_par;                          // rows that its threads take at once
   int gb, slabs;                         // slab: groups of a workgroup, workgroups of an image
   int chunks, rows_chunk, tiles;         // split
+  int stat_par;                          // rows that a statistics workgroup's threads take at once
 };
 
 // VEC consecutive values of a row as one load: 16 bytes where the pointers and strides allow it, 4 bytes or one value otherwise
@@ -263,7 +264,7 @@ __global__ __launch_bounds__(512, gn_slab_waves(R, VEC * (int)sizeof(T))) void g
 // ---- split -----------------------------------------------------------------------------------------------------------------------
 // Channel tiles of cv vectors x chunks of rows_chunk positions.  Group g's part of tile t stands at place g + t of a chunk's
 // row of parts: neighbouring tiles share at most one group, so no two parts meet.
-constexpr int kGnThreads = 256, kGnBatch = 8;
+constexpr int kGnThreads = 256, kGnStatThreads = 512, kGnBatch = 8;
 
 struct GnPlace {
   long img;
@@ -288,23 +289,23 @@ __device__ __forceinline__ GnPlace gn_place(const GnArgs& a, int chunks) {
 // Statistics: every thread takes one vector of channels over every rows_par-th position of the chunk, eight at a time;
 // differences are summed from the mean of its first eight, so that the squares cannot cancel.
 template <typename T, int VEC>
-__global__ __launch_bounds__(256, 5) void gn_stats_kernel(const GnArgs a) {
+__global__ __launch_bounds__(512, 4) void gn_stats_kernel(const GnArgs a) {
   typedef GnVec<T, VEC> V;
-  __shared__ float lm[kGnThreads * VEC], lq[kGnThreads * VEC];
+  __shared__ float lm[kGnStatThreads * VEC], lq[kGnStatThreads * VEC];
   const GnPlace p = gn_place<VEC>(a, a.chunks);
   const long rows = gn_rows(a, p.img);
   const long r0 = (long)p.chunk * a.rows_chunk, r1 = r0 + a.rows_chunk < rows ? r0 + a.rows_chunk : rows;
   if (r0 >= r1) return;
   const int tid = (int)threadIdx.x, rp = tid / a.cv, col = tid - rp * a.cv;
   const int ch = p.ch0 + col * VEC;
-  const bool on = rp < a.rows_par && ch < a.c;
+  const bool on = rp < a.stat_par && ch < a.c;
   // thread rows hold each_has positions of the chunk, the first `over` of them one more
-  const int nrows = (int)(r1 - r0), each_has = nrows / a.rows_par, over = nrows - each_has * a.rows_par;
+  const int nrows = (int)(r1 - r0), each_has = nrows / a.stat_par, over = nrows - each_has * a.stat_par;
   // (threads without a vector or a thread row read the first ones again, uncounted: no load is conditional)
-  const int row = rp < a.rows_par && rp < nrows ? rp : 0;
+  const int row = rp < a.stat_par && rp < nrows ? rp : 0;
   const T* const x0 = (const T*)a.x + p.img * a.x_image + (on ? ch : p.ch0) + r0 * a.x_row;
   const T* x = x0 + row * a.x_row;
-  const long step = a.rows_par * a.x_row;
+  const long step = a.stat_par * a.x_row;
   float piv[VEC], s1[VEC], s2[VEC];
 #pragma unroll
   for (int e = 0; e < VEC; ++e) piv[e] = s1[e] = s2[e] = 0.0f;
@@ -348,7 +349,7 @@ __global__ __launch_bounds__(256, 5) void gn_stats_kernel(const GnArgs a) {
   auto count = [&](int k) { return (float)(each_has + (k < over ? 1 : 0)); };     // positions of thread row k
   {
     const float n = count(rp), inv = n > 0.0f ? 1.0f / n : 0.0f;
-    if (rp < a.rows_par) {
+    if (rp < a.stat_par) {
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
         const float q = s2[e] - s1[e] * s1[e] * inv;
@@ -358,9 +359,9 @@ __global__ __launch_bounds__(256, 5) void gn_stats_kernel(const GnArgs a) {
     }
   }
   __syncthreads();
-  const int lanes = gn_lanes(kGnThreads, p.groups), j = tid & (lanes - 1), width = a.cv * VEC;
-  const int thread_rows = r1 - r0 < a.rows_par ? (int)(r1 - r0) : a.rows_par;     // thread rows that have a position
-  for (int gl = 0; gl < p.groups; gl += kGnThreads / lanes) {
+  const int lanes = gn_lanes(kGnStatThreads, p.groups), j = tid & (lanes - 1), width = a.cv * VEC;
+  const int thread_rows = r1 - r0 < a.stat_par ? (int)(r1 - r0) : a.stat_par;     // thread rows that have a position
+  for (int gl = 0; gl < p.groups; gl += kGnStatThreads / lanes) {
     const int g = gl + tid / lanes;
     int from = (p.g0 + g) * a.cg - p.ch0, to = from + a.cg;     // the group's channels in the tile
     if (from < 0) from = 0;
@@ -404,31 +405,55 @@ __global__ __launch_bounds__(256, 6) void gn_apply_kernel(const GnArgs a, int ch
   const int ch = p.ch0 + col * VEC;
   const bool on = rp < a.rows_par && ch < a.c;
   const int lanes = gn_lanes(kGnThreads, p.groups), j = tid & (lanes - 1);
-  const int slots = a.groups + a.tiles - 1;
+  const int slots = a.groups + a.tiles - 1, tile_c = a.cv * VEC;
+  const int nv = (int)((rows + a.rows_chunk - 1) / a.rows_chunk);       // chunks that have positions, and left parts
+  const float last = (float)(rows - (long)(nv - 1) * a.rows_chunk), each = (float)a.rows_chunk;
   for (int gl = 0; gl < p.groups; gl += kGnThreads / lanes) {
     const int g = gl + tid / lanes;
     const bool mine = g < p.groups;
-    const int c0 = (p.g0 + (mine ? g : 0)) * a.cg, t0 = c0 / (a.cv * VEC), t1 = (c0 + a.cg - 1) / (a.cv * VEC);
-    const float2* const part = a.part + p.img * a.chunks * (long)slots + p.g0 + g;
-    const float m0 = mine ? ld(&part[t0]).x : 0.0f;
-    auto each = [&](auto f) {
-      if (!mine) return;
-      for (int t = t0; t <= t1; ++t) {
-        const int lo = c0 > t * a.cv * VEC ? c0 : t * a.cv * VEC;
-        const int hi = c0 + a.cg < (t + 1) * a.cv * VEC ? c0 + a.cg : (t + 1) * a.cv * VEC;
-        for (int k = j; k < a.chunks; k += lanes) {
-          long in = rows - (long)k * a.rows_chunk;
-          if (in <= 0) break;                                     // (a chunk behind the image's length left no part)
-          in = in < a.rows_chunk ? in : a.rows_chunk;
-          f((float)in * (float)(hi - lo), ld(part + (long)k * slots + t));
-        }
+    const int c0 = (p.g0 + (mine ? g : 0)) * a.cg, t0 = c0 / tile_c, t1 = (c0 + a.cg - 1) / tile_c;
+    const float2* const part = a.part + p.img * a.chunks * (long)slots + p.g0 + (mine ? g : 0) + t0;
+    const float m0 = ld(part).x, total = (float)rows * (float)a.cg;
+    float t = 0.0f, q = 0.0f, m;
+    if (a.tiles == 1) {
+      // a lane's first parts stay in registers; their loads are one wait
+      constexpr int HELD = 4;
+      float2 v[HELD];
+      float n[HELD];
+#pragma unroll
+      for (int i = 0; i < HELD; ++i) {
+        const int k = j + i * lanes;
+        v[i] = ld(part + (long)(k < nv ? k : nv - 1) * slots);
+        n[i] = k < nv - 1 ? each : k == nv - 1 ? last : 0.0f;
       }
-    };
-    float t = 0.0f, q = 0.0f;
-    each([&](float n, float2 v) { t += n * (v.x - m0); });
-    t = gn_lane_sum(t, lanes);
-    const float total = (float)rows * (float)a.cg, m = m0 + t / total;
-    each([&](float n, float2 v) { q += v.y + n * (v.x - m) * (v.x - m); });
+#pragma unroll
+      for (int i = 0; i < HELD; ++i) t += n[i] * (v[i].x - m0);
+      for (int k = j + HELD * lanes; k < nv; k += lanes) t += (k < nv - 1 ? each : last) * (ld(part + (long)k * slots).x - m0);
+      t = gn_lane_sum(t, lanes);
+      m = m0 + t / (float)rows;
+#pragma unroll
+      for (int i = 0; i < HELD; ++i) {
+        const float d = v[i].x - m;
+        if (n[i] > 0.0f) q += v[i].y + n[i] * (float)a.cg * d * d;
+      }
+      for (int k = j + HELD * lanes; k < nv; k += lanes) {
+        const float2 o = ld(part + (long)k * slots);
+        q += o.y + (k < nv - 1 ? each : last) * (float)a.cg * (o.x - m) * (o.x - m);
+      }
+    } else {
+      // (a group's channels in several tiles: a part of each)
+      auto all = [&](auto f) {
+        for (int dt = 0; dt <= t1 - t0; ++dt) {
+          const int lo = (t0 + dt) * tile_c, hi = lo + tile_c;
+          const float w = (float)((c0 + a.cg < hi ? c0 + a.cg : hi) - (c0 > lo ? c0 : lo));
+          for (int k = j; k < nv; k += lanes) f((k < nv - 1 ? each : last) * w, ld(part + (long)k * slots + dt));
+        }
+      };
+      all([&](float n, float2 o) { t += n * (o.x - m0); });
+      t = gn_lane_sum(t, lanes);
+      m = m0 + t / total;
+      all([&](float n, float2 o) { q += o.y + n * (o.x - m) * (o.x - m); });
+    }
     q = gn_lane_sum(q, lanes);
     if (mine && j == 0) {
       mean[g] = m;
@@ -455,7 +480,7 @@ __global__ __launch_bounds__(256, 6) void gn_apply_kernel(const GnArgs a, int ch
 #pragma unroll
     for (int e = 0; e < VEC; ++e) v[e] = (v[e] - m[e]) * sc[e] + sh[e];
     gn_activate(v, a.act);
-    st((typename V::raw*)to, V::put(v));
+    st_stream((typename V::raw*)to, V::put(v));
   };
   constexpr int U = kGnBatch / 2;
   int i = 0;
@@ -524,8 +549,9 @@ static int gn_launch(const eco_group_norm_plan& p, GnArgs& a, hipStream_t st) {
   a.cv = (int)ceil_div(vecs, a.tiles);
   a.tiles = (int)ceil_div(vecs, a.cv);
   a.rows_par = kGnThreads / a.cv;
+  a.stat_par = kGnStatThreads / a.cv;
   // (chunks of whole batches, so no more of them than the plan's)
-  a.rows_chunk = (int)(ceil_div(ceil_div(p.s, p.chunks), kGnBatch * a.rows_par) * kGnBatch * a.rows_par);
+  a.rows_chunk = (int)(ceil_div(ceil_div(p.s, p.chunks), kGnBatch * a.stat_par) * kGnBatch * a.stat_par);
   a.chunks = (int)ceil_div(p.s, a.rows_chunk);
   const long parts = p.n * a.chunks * a.tiles;
   // result: eight workgroups a compute unit, of whole batches of positions
@@ -534,7 +560,7 @@ static int gn_launch(const eco_group_norm_plan& p, GnArgs& a, hipStream_t st) {
   const long chunks = ceil_div(p.s, rows_chunk);
   const long results = p.n * chunks * a.tiles;
   ECO_REQUIRE(parts <= 2147483647l && results <= 2147483647l, "group_norm: too many positions, images and channels for one launch");
-  hipLaunchKernelGGL((gn_stats_kernel<T, VEC>), dim3((unsigned)parts), dim3(kGnThreads), 0, st, a);
+  hipLaunchKernelGGL((gn_stats_kernel<T, VEC>), dim3((unsigned)parts), dim3(kGnStatThreads), 0, st, a);
   if (int rc = check_launch("eco_group_norm_forward(statistics)")) return rc;
   hipLaunchKernelGGL((gn_apply_kernel<T, VEC>), dim3((unsigned)results), dim3(kGnThreads), 0, st, a, (int)chunks, rows_chunk);
   return check_launch("eco_group_norm_forward");
@@ -564,10 +590,10 @@ extern "C" int eco_group_norm_plan_create(int64_t n, int64_t s, int32_t c, int32
   const bool always = gn_slab_fits(s, cg, groups, 1, es, &sl) && (c % wide || gn_slab_fits(s, cg, groups, wide, es, &sl)) &&
                       (es == 4 || c % 2 || gn_slab_fits(s, cg, groups, 2, es, &sl));
   if (always) return ECO_OK;
-  // statistics: eight workgroups a compute unit, of a batch of positions a thread at least
+  // statistics: four workgroups a compute unit, of a batch of positions a thread at least
   const long vecs = c % wide ? c : c / wide, tiles = ceil_div(vecs, kGnThreads);
-  const long rows_par = kGnThreads / ceil_div(vecs, tiles);
-  long chunks = ceil_div(8l * plan->num_cu, n * tiles);
+  const long rows_par = kGnStatThreads / ceil_div(vecs, tiles);
+  long chunks = ceil_div(4l * plan->num_cu, n * tiles);
   const long most = ceil_div(s, kGnBatch * rows_par);
   if (chunks > most) chunks = most;
   if (chunks > kGnMaxChunks) chunks = kGnMaxChunks;

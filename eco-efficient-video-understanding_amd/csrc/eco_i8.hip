@@ -7,9 +7,6 @@ namespace eco {
 
 constexpr int kI8Threads = 256;
 
-__device__ __forceinline__ float i8_load(const float* p) { return ld(p); }
-__device__ __forceinline__ float i8_load(const unsigned short* p) { return bf16_bits_to_f32(ld(p)); }
-
 __device__ __forceinline__ unsigned f32_bits(float v) {
   unsigned u;
   __builtin_memcpy(&u, &v, 4);
@@ -21,47 +18,247 @@ __device__ __forceinline__ float bits_f32(unsigned u) {
   return v;
 }
 
-// The integer nearest to 127 v / top (ties to even), 0 <= |v| <= top, top > 0 and finite.  inv = fp32(127 / top): the product
-// is off by at most 127 * 2^-23 = 1.6e-5, so its rounding is right unless it lies within 1e-4 of a half; there the sides of
-// the comparison |v| * 254 <> (2 k + 1) * top are products of a 24-bit and an 8-bit number, exact in fp64.
-__device__ __forceinline__ int i8_quant(float v, float top, float inv) {
-  const float t = v * inv;
-  const float r = rintf(t);
-  if (fabsf(fabsf(t - r) - 0.5f) > 1e-4f) return (int)r;
-  const float k = floorf(fabsf(t));
-  const double lhs = fabs((double)v) * 254.0, rhs = (double)(2.0f * k + 1.0f) * (double)top;
-  const int n = (int)k + ((lhs > rhs || (lhs == rhs && ((int)k & 1))) ? 1 : 0);
-  return v < 0.0f ? -n : n;
+// ---- rows to integers ----------------------------------------------------------------------------------------------------------
+// Bound by memory: a row is read once into registers, its largest magnitude found as bits (a NaN or an infinity has the largest),
+// and its integers written.
+//
+// The integers are those of the exact quotient 127 v / top.  In fp32 t = v * inv with inv = 127 * (1 / top) from the hardware's
+// reciprocal is off by at most 127 * 4 * 2^-24 = 3.1e-5, so rint(t) is right unless t lies within 1e-4 of a half; there, and in
+// rows of tiny or huge values (127 / top or 1 / top would leave fp32's normal range), the quotient is taken in fp64: 127 v has 31 bits and top has 24, so a
+// quotient that is no tie is at least 2^-32 of itself away from one and fp64's rounding cannot cross it.
+__device__ __forceinline__ int quant_exact(float v, float top) { return (int)rint((double)v * 127.0 / (double)top); }
+
+template <int VEC>
+struct QuantRow {     // what a row's lanes share once its largest magnitude is known
+  float top, inv, scale;
+  bool live, far;     // integers other than 0; the fp64 way for all of them
+  __device__ __forceinline__ explicit QuantRow(unsigned top_bits) {
+    const bool finite = top_bits < 0x7f800000u;
+    top = bits_f32(top_bits);
+    scale = finite ? top / 127.0f : bits_f32(0x7fc00000u);
+    live = finite && top_bits != 0u;
+    far = top < 1e-30f || top > 1e37f;
+#ifdef ECO_EMU
+    inv = 127.0f * (1.0f / top);
+#else
+    inv = 127.0f * __builtin_amdgcn_rcpf(top);
+#endif
+  }
+  __device__ __forceinline__ void integers(const float (&v)[VEC], int (&q)[VEC]) const {
+    float off = 0.0f;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      const float t = v[e] * inv, r = rintf(t);
+      off = fmaxf(off, fabsf(t - r));
+      q[e] = (int)r;
+    }
+    if (live && (far || off > 0.4999f)) {
+#pragma unroll 1
+      for (int e = 0; e < VEC; ++e) {      // (rare: one rolled copy; the values pass through registers by selection)
+        float x = v[0];
+#pragma unroll
+        for (int u = 1; u < VEC; ++u) x = u == e ? v[u] : x;
+        const int n = quant_exact(x, top);
+#pragma unroll
+        for (int u = 0; u < VEC; ++u) q[u] = u == e ? n : q[u];
+      }
+    }
+    if (!live) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) q[e] = 0;
+    }
+  }
+};
+
+template <typename T, int VEC>
+struct QuantVec;
+template <>
+struct QuantVec<float, 4> {
+  typedef uint4 raw;
+  static __device__ __forceinline__ void get(const raw& r, float (&v)[4]) { __builtin_memcpy(v, &r, 16); }
+};
+template <>
+struct QuantVec<unsigned short, 8> {
+  typedef uint4 raw;
+  static __device__ __forceinline__ void get(const raw& r, float (&v)[8]) {
+    const unsigned w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] = bf16_bits_to_f32(w[i] & 0xffffu);
+      v[2 * i + 1] = bf16_bits_to_f32(w[i] >> 16);
+    }
+  }
+};
+template <>
+struct QuantVec<float, 1> {
+  typedef float raw;
+  static __device__ __forceinline__ void get(const raw& r, float (&v)[1]) { v[0] = r; }
+};
+template <>
+struct QuantVec<unsigned short, 1> {
+  typedef unsigned short raw;
+  static __device__ __forceinline__ void get(const raw& r, float (&v)[1]) { v[0] = bf16_bits_to_f32(r); }
+};
+
+template <int VEC>
+__device__ __forceinline__ unsigned quant_top(const float (&v)[VEC], unsigned top) {
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) {
+    const unsigned b = f32_bits(v[e]) & 0x7fffffffu;
+    top = b > top ? b : top;
+  }
+  return top;
+}
+__device__ __forceinline__ unsigned quant_lanes_top(unsigned top, int lanes) {
+  for (int d = lanes >> 1; d >= 1; d >>= 1) {
+    const unsigned o = f32_bits(shfl_xor(bits_f32(top), d));
+    top = o > top ? o : top;
+  }
+  return top;
+}
+__device__ __forceinline__ unsigned pack_i8x4(int a, int b, int c, int d) {
+  return ((unsigned)a & 0xffu) | (((unsigned)b & 0xffu) << 8) | (((unsigned)c & 0xffu) << 16) | ((unsigned)d << 24);
+}
+template <int VEC>
+__device__ __forceinline__ void quant_store(signed char* q, const int (&n)[VEC]) {
+  if constexpr (VEC == 8) st((uint2*)q, make_uint2(pack_i8x4(n[0], n[1], n[2], n[3]), pack_i8x4(n[4], n[5], n[6], n[7])));
+  else if constexpr (VEC == 4) st((unsigned*)q, pack_i8x4(n[0], n[1], n[2], n[3]));
+  else st(q, (signed char)n[0]);
 }
 
-// One wave per row: the largest magnitude as bits (a NaN or an infinity has the largest), then the integers.
-template <typename T>
-__global__ __launch_bounds__(256) void quant_rows_kernel(const T* x, long ldx, signed char* q, long ldq, float* scale,
-                                                         long m, long k) {
-  const int lane = lane_id();
-  const int wave = uniform((int)(threadIdx.x >> 6));
-  for (long i = (long)blockIdx.x * 4 + wave; i < m; i += (long)gridDim.x * 4) {
-    const T* xr = x + i * ldx;
-    unsigned top_bits = 0u;
-    for (long j = lane; j < k; j += kWave) {
-      const unsigned b = f32_bits(i8_load(xr + j)) & 0x7fffffffu;
-      top_bits = b > top_bits ? b : top_bits;
-    }
+struct QuantArgs {
+  const void* x;
+  signed char* q;
+  float* scale;
+  long ldx, ldq, m, k;
+  int nv;        // vectors of a row
+  int lanes;     // lanes of a row (power of two up to 64)
+};
+
+// Rows of up to 64 vectors: `lanes` lanes take a row, a vector each; a wave takes ROWS sets of 64 / lanes rows, all loaded at once.
+constexpr int kQuantSets = 4;
+template <typename T, int VEC>
+__global__ __launch_bounds__(256) void quant_short_kernel(const QuantArgs a) {
+  typedef QuantVec<T, VEC> V;
+  const int lane = lane_id(), per = kWave / a.lanes, sub = lane / a.lanes, j = lane & (a.lanes - 1);
+  const long wave = (long)blockIdx.x * 4 + uniform((int)(threadIdx.x >> 6));
+  const long r0 = wave * kQuantSets * per + sub;
+  const int jv = j < a.nv ? j : a.nv - 1;
+  typename V::raw raw[kQuantSets];
 #pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) {
-      const unsigned o = f32_bits(shfl_xor(bits_f32(top_bits), d));
-      top_bits = o > top_bits ? o : top_bits;
-    }
-    const bool finite = top_bits < 0x7f800000u;
-    float top = bits_f32(top_bits);
-    if (lane == 0) st(scale + i, finite ? top / 127.0f : bits_f32(0x7fc00000u));
-    // rows of tiny values are scaled up by a power of two first: 127 / top must be finite
-    const float up = top < 1e-30f ? 1.2676506e30f : 1.0f;   // 2^100
-    top *= up;
-    const float inv = 127.0f / top;
-    for (long j = lane; j < k; j += kWave)
-      st(q + i * ldq + j, (signed char)(finite && top > 0.0f ? i8_quant(i8_load(xr + j) * up, top, inv) : 0));
+  for (int s = 0; s < kQuantSets; ++s) {
+    const long row = r0 + s * per < a.m ? r0 + s * per : a.m - 1;      // (behind the last row: its values again, not stored)
+    raw[s] = ld((const typename V::raw*)((const T*)a.x + row * a.ldx + (long)jv * VEC));
   }
+#pragma unroll
+  for (int s = 0; s < kQuantSets; ++s) {
+    const long row = r0 + s * per;
+    float v[VEC];
+    int n[VEC];
+    V::get(raw[s], v);
+    const QuantRow<VEC> qr(quant_lanes_top(quant_top(v, 0u), a.lanes));
+    qr.integers(v, n);
+    if (row < a.m) {
+      if (j < a.nv) quant_store(a.q + row * a.ldq + (long)j * VEC, n);
+      if (j == 0) st(a.scale + row, qr.scale);
+    }
+  }
+}
+
+// Longer rows: a workgroup of 256 or 1024 threads (one wave: four rows a workgroup) takes a row, R vectors a thread in registers.
+template <typename T, int VEC, int R, int NT>
+__global__ __launch_bounds__(NT < 256 ? 256 : NT) void quant_row_kernel(const QuantArgs a) {
+  typedef QuantVec<T, VEC> V;
+  __shared__ unsigned tops[NT / kWave];
+  const int tid = NT == kWave ? lane_id() : (int)threadIdx.x;
+  const long row = NT == kWave ? (long)blockIdx.x * 4 + uniform((int)(threadIdx.x >> 6)) : (long)blockIdx.x;
+  if (row >= a.m) return;                     // (whole waves; with one row a workgroup never)
+  const T* const x = (const T*)a.x + row * a.ldx;
+  typename V::raw raw[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const int at = tid + i * NT;
+    raw[i] = ld((const typename V::raw*)(x + (long)(at < a.nv ? at : a.nv - 1) * VEC));
+  }
+  unsigned top = 0u;
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    float v[VEC];
+    V::get(raw[i], v);
+    top = quant_top(v, top);
+  }
+  top = quant_lanes_top(top, kWave);
+  if constexpr (NT > kWave) {
+    if (lane_id() == 0) tops[threadIdx.x >> 6] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < NT / kWave; ++w) top = tops[w] > top ? tops[w] : top;
+  }
+  const QuantRow<VEC> qr(top);
+  if (tid == 0) st(a.scale + row, qr.scale);
+  signed char* const q = a.q + row * a.ldq;
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const int at = tid + i * NT;
+    if (at < a.nv) {
+      float v[VEC];
+      int n[VEC];
+      V::get(raw[i], v);
+      qr.integers(v, n);
+      quant_store(q + (long)at * VEC, n);
+    }
+  }
+}
+
+// Rows that no workgroup's registers hold: read twice.
+template <typename T, int VEC>
+__global__ __launch_bounds__(1024) void quant_long_kernel(const QuantArgs a) {
+  typedef QuantVec<T, VEC> V;
+  __shared__ unsigned tops[16];
+  const T* const x = (const T*)a.x + (long)blockIdx.x * a.ldx;
+  unsigned top = 0u;
+  for (int at = (int)threadIdx.x; at < a.nv; at += 1024) {
+    float v[VEC];
+    V::get(ld((const typename V::raw*)(x + (long)at * VEC)), v);
+    top = quant_top(v, top);
+  }
+  top = quant_lanes_top(top, kWave);
+  if (lane_id() == 0) tops[threadIdx.x >> 6] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 16; ++w) top = tops[w] > top ? tops[w] : top;
+  const QuantRow<VEC> qr(top);
+  if (threadIdx.x == 0) st(a.scale + (long)blockIdx.x, qr.scale);
+  for (int at = (int)threadIdx.x; at < a.nv; at += 1024) {
+    float v[VEC];
+    int n[VEC];
+    V::get(ld((const typename V::raw*)(x + (long)at * VEC)), v);
+    qr.integers(v, n);
+    quant_store(a.q + (long)blockIdx.x * a.ldq + (long)at * VEC, n);
+  }
+}
+
+template <typename T, int VEC>
+static int quant_launch(QuantArgs& a, hipStream_t st) {
+  a.nv = (int)(a.k / VEC);
+  const unsigned m = (unsigned)a.m;
+  if (a.nv <= kWave) {
+    a.lanes = 1;
+    while (a.lanes < a.nv) a.lanes *= 2;
+    const long rows = 4l * kQuantSets * (kWave / a.lanes);           // of a workgroup
+    hipLaunchKernelGGL((quant_short_kernel<T, VEC>), dim3((unsigned)ceil_div(a.m, rows)), dim3(256), 0, st, a);
+  } else if (a.nv <= kWave * 4) {
+    hipLaunchKernelGGL((quant_row_kernel<T, VEC, 4, 64>), dim3((unsigned)ceil_div(a.m, 4)), dim3(256), 0, st, a);
+  } else if (a.nv <= 256 * 4) {
+    hipLaunchKernelGGL((quant_row_kernel<T, VEC, 4, 256>), dim3(m), dim3(256), 0, st, a);
+  } else if (a.nv <= 256 * 8) {
+    hipLaunchKernelGGL((quant_row_kernel<T, VEC, 8, 256>), dim3(m), dim3(256), 0, st, a);
+  } else if (a.nv <= 1024 * 8) {
+    hipLaunchKernelGGL((quant_row_kernel<T, VEC, 8, 1024>), dim3(m), dim3(1024), 0, st, a);
+  } else {
+    hipLaunchKernelGGL((quant_long_kernel<T, VEC>), dim3(m), dim3(1024), 0, st, a);
+  }
+  return check_launch("eco_quant_rows_forward");
 }
 
 struct I8Args {
@@ -594,15 +791,15 @@ extern "C" int eco_quant_rows_forward(const void* x, int32_t dt, int64_t ldx, in
   if (ldq == 0) ldq = k;
   ECO_REQUIRE(ldx >= k && ldq >= k, "quant_rows: a row stride is smaller than %ld", (long)k);
   ECO_REQUIRE(extent_fits(m, ldx, k) && extent_fits(m, ldq, k), "quant_rows: a row stride is too large");
+  QuantArgs a;
+  memset(&a, 0, sizeof(a));
+  a.x = x; a.q = (signed char*)q; a.scale = scale; a.ldx = ldx; a.ldq = ldq; a.m = m; a.k = k;
   hipStream_t st = (hipStream_t)stream;
-  const dim3 grid(i8_grid(m, 4)), block(kI8Threads);
-  if (dt == ECO_DT_F32)
-    hipLaunchKernelGGL((quant_rows_kernel<float>), grid, block, 0, st, (const float*)x, (long)ldx, (signed char*)q, (long)ldq,
-                       scale, (long)m, (long)k);
-  else
-    hipLaunchKernelGGL((quant_rows_kernel<unsigned short>), grid, block, 0, st, (const unsigned short*)x, (long)ldx,
-                       (signed char*)q, (long)ldq, scale, (long)m, (long)k);
-  return check_launch("eco_quant_rows_forward");
+  // vectors of 16 bytes where rows and both pointers allow them, single values otherwise
+  const int vec = 16 / (int)es;
+  const bool wide = k % vec == 0 && ldx % vec == 0 && (uintptr_t)x % 16 == 0 && ldq % vec == 0 && (uintptr_t)q % vec == 0;
+  if (dt == ECO_DT_F32) return wide ? quant_launch<float, 4>(a, st) : quant_launch<float, 1>(a, st);
+  return wide ? quant_launch<unsigned short, 8>(a, st) : quant_launch<unsigned short, 1>(a, st);
 }
 
 extern "C" int eco_inner_product_i8_plan_create(int64_t m, int64_t n, int64_t k, int32_t dt, int32_t num_cu,

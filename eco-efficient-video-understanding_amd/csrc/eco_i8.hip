@@ -22,10 +22,11 @@ __device__ __forceinline__ float bits_f32(unsigned u) {
 // Bound by memory: a row is read once into registers, its largest magnitude found as bits (a NaN or an infinity has the largest),
 // and its integers written.
 //
-// The integers are those of the exact quotient 127 v / top.  In fp32 t = v * inv with inv = 127 * (1 / top) from the hardware's
-// reciprocal is off by at most 127 * 4 * 2^-24 = 3.1e-5, so rint(t) is right unless t lies within 1e-4 of a half; there, and in
-// rows of tiny or huge values (127 / top or 1 / top would leave fp32's normal range), the quotient is taken in fp64: 127 v has 31 bits and top has 24, so a
-// quotient that is no tie is at least 2^-32 of itself away from one and fp64's rounding cannot cross it.
+// The integers are those of the exact quotient 127 v / top.  In fp32, v * inv with inv = 127 * (1 / top) from the hardware's
+// reciprocal is off by at most 127 * 2^-22 = 3.03e-5 (reciprocal 2^-23, its product 2^-24, and the rest of its slack), so its
+// nearest integer is right unless it lies within 4e-5 of a half; there, and in rows of tiny or huge values (127 / top or 1 / top
+// would leave fp32's normal range), the quotient is taken in fp64: 127 v has 31 bits and top has 24, so a quotient that is no
+// tie is at least 2^-32 of itself away from one and fp64's rounding cannot cross it.
 __device__ __forceinline__ int quant_exact(float v, float top) { return (int)rint((double)v * 127.0 / (double)top); }
 
 template <int VEC>
@@ -44,42 +45,62 @@ struct QuantRow {     // what a row's lanes share once its largest magnitude is 
     inv = 127.0f * __builtin_amdgcn_rcpf(top);
 #endif
   }
-  __device__ __forceinline__ void integers(const float (&v)[VEC], int (&q)[VEC]) const {
-    float off = 0.0f;
+  // Bits whose low byte is the integer: v * inv + 1.5 * 2^23 rounds the product (unrounded before) to the nearest integer,
+  // ties to even, and leaves it in the low bits.
+  __device__ __forceinline__ void integers(const float (&v)[VEC], unsigned (&q)[VEC]) const {
+    constexpr float kMagic = 12582912.0f;
+    float off[VEC], most = 0.0f;
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
-      const float t = v[e] * inv, r = rintf(t);
-      off = fmaxf(off, fabsf(t - r));
-      q[e] = (int)r;
+      const float u = __builtin_fmaf(v[e], inv, kMagic);
+      off[e] = __builtin_fmaf(v[e], inv, -(u - kMagic));
+      most = fmaxf(most, fabsf(off[e]));
+      q[e] = f32_bits(u);
     }
-    if (live && (far || off > 0.4999f)) {
-#pragma unroll 1
-      for (int e = 0; e < VEC; ++e) {      // (rare: one rolled copy; the values pass through registers by selection)
-        float x = v[0];
+    if (live && (far || most > 0.49996f)) {
 #pragma unroll
-        for (int u = 1; u < VEC; ++u) x = u == e ? v[u] : x;
-        const int n = quant_exact(x, top);
-#pragma unroll
-        for (int u = 0; u < VEC; ++u) q[u] = u == e ? n : q[u];
-      }
+      for (int e = 0; e < VEC; ++e)
+        if (far || fabsf(off[e]) > 0.49996f) q[e] = (unsigned)quant_exact(v[e], top);
     }
     if (!live) {
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) q[e] = 0;
+      for (int e = 0; e < VEC; ++e) q[e] = 0u;
     }
   }
 };
 
+// (the larger of a running magnitude and a value's, as bits)
+__device__ __forceinline__ unsigned quant_top(unsigned v, unsigned t) {
+  v &= 0x7fffffffu;
+  return v > t ? v : t;
+}
+// A row's values as loads of 16 bytes or one: top() gathers magnitudes, bits() is the largest of them as fp32 bits
 template <typename T, int VEC>
 struct QuantVec;
 template <>
 struct QuantVec<float, 4> {
   typedef uint4 raw;
+  static __device__ __forceinline__ unsigned top(const raw& r, unsigned t) { return quant_top(r.w, quant_top(r.z, quant_top(r.y, quant_top(r.x, t)))); }
+  static __device__ __forceinline__ unsigned bits(unsigned t) { return t; }
   static __device__ __forceinline__ void get(const raw& r, float (&v)[4]) { __builtin_memcpy(v, &r, 16); }
 };
 template <>
 struct QuantVec<unsigned short, 8> {
   typedef uint4 raw;
+  // (pairs of magnitudes, the largest of either half)
+  static __device__ __forceinline__ unsigned top(const raw& r, unsigned t) { return pair_max(pair_max(r.x, r.y), pair_max(pair_max(r.z, r.w), t)); }
+  static __device__ __forceinline__ unsigned pair_max(unsigned a, unsigned b) {
+    typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+    a &= 0x7fff7fffu;
+    b &= 0x7fff7fffu;
+    u16x2 x, y;
+    __builtin_memcpy(&x, &a, 4);
+    __builtin_memcpy(&y, &b, 4);
+    x = __builtin_elementwise_max(x, y);
+    __builtin_memcpy(&a, &x, 4);
+    return a;
+  }
+  static __device__ __forceinline__ unsigned bits(unsigned t) { return (t << 16) > (t & 0xffff0000u) ? t << 16 : t & 0xffff0000u; }
   static __device__ __forceinline__ void get(const raw& r, float (&v)[8]) {
     const unsigned w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
@@ -92,23 +113,18 @@ struct QuantVec<unsigned short, 8> {
 template <>
 struct QuantVec<float, 1> {
   typedef float raw;
+  static __device__ __forceinline__ unsigned top(const raw& r, unsigned t) { return quant_top(f32_bits(r), t); }
+  static __device__ __forceinline__ unsigned bits(unsigned t) { return t; }
   static __device__ __forceinline__ void get(const raw& r, float (&v)[1]) { v[0] = r; }
 };
 template <>
 struct QuantVec<unsigned short, 1> {
   typedef unsigned short raw;
+  static __device__ __forceinline__ unsigned top(const raw& r, unsigned t) { return quant_top((unsigned)r << 16, t); }
+  static __device__ __forceinline__ unsigned bits(unsigned t) { return t; }
   static __device__ __forceinline__ void get(const raw& r, float (&v)[1]) { v[0] = bf16_bits_to_f32(r); }
 };
 
-template <int VEC>
-__device__ __forceinline__ unsigned quant_top(const float (&v)[VEC], unsigned top) {
-#pragma unroll
-  for (int e = 0; e < VEC; ++e) {
-    const unsigned b = f32_bits(v[e]) & 0x7fffffffu;
-    top = b > top ? b : top;
-  }
-  return top;
-}
 __device__ __forceinline__ unsigned quant_lanes_top(unsigned top, int lanes) {
   for (int d = lanes >> 1; d >= 1; d >>= 1) {
     const unsigned o = f32_bits(shfl_xor(bits_f32(top), d));
@@ -116,13 +132,19 @@ __device__ __forceinline__ unsigned quant_lanes_top(unsigned top, int lanes) {
   }
   return top;
 }
-__device__ __forceinline__ unsigned pack_i8x4(int a, int b, int c, int d) {
-  return ((unsigned)a & 0xffu) | (((unsigned)b & 0xffu) << 8) | (((unsigned)c & 0xffu) << 16) | ((unsigned)d << 24);
+// The low bytes of four words.
+__device__ __forceinline__ unsigned pack_low_bytes(unsigned a, unsigned b, unsigned c, unsigned d) {
+#ifdef ECO_EMU
+  return (a & 0xffu) | ((b & 0xffu) << 8) | ((c & 0xffu) << 16) | (d << 24);
+#else
+  // v_perm_b32 picks bytes of its second operand as 0 .. 3 and of its first as 4 .. 7
+  return __builtin_amdgcn_perm(__builtin_amdgcn_perm(d, c, 0x0c0c0400u), __builtin_amdgcn_perm(b, a, 0x0c0c0400u), 0x05040100u);
+#endif
 }
 template <int VEC>
-__device__ __forceinline__ void quant_store(signed char* q, const int (&n)[VEC]) {
-  if constexpr (VEC == 8) st((uint2*)q, make_uint2(pack_i8x4(n[0], n[1], n[2], n[3]), pack_i8x4(n[4], n[5], n[6], n[7])));
-  else if constexpr (VEC == 4) st((unsigned*)q, pack_i8x4(n[0], n[1], n[2], n[3]));
+__device__ __forceinline__ void quant_store(signed char* q, const unsigned (&n)[VEC]) {
+  if constexpr (VEC == 8) st((uint2*)q, make_uint2(pack_low_bytes(n[0], n[1], n[2], n[3]), pack_low_bytes(n[4], n[5], n[6], n[7])));
+  else if constexpr (VEC == 4) st((unsigned*)q, pack_low_bytes(n[0], n[1], n[2], n[3]));
   else st(q, (signed char)n[0]);
 }
 
@@ -154,9 +176,9 @@ __global__ __launch_bounds__(256) void quant_short_kernel(const QuantArgs a) {
   for (int s = 0; s < kQuantSets; ++s) {
     const long row = r0 + s * per;
     float v[VEC];
-    int n[VEC];
+    unsigned n[VEC];
+    const QuantRow<VEC> qr(quant_lanes_top(V::bits(V::top(raw[s], 0u)), a.lanes));
     V::get(raw[s], v);
-    const QuantRow<VEC> qr(quant_lanes_top(quant_top(v, 0u), a.lanes));
     qr.integers(v, n);
     if (row < a.m) {
       if (j < a.nv) quant_store(a.q + row * a.ldq + (long)j * VEC, n);
@@ -182,12 +204,8 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void quant_row_kernel(const Qu
   }
   unsigned top = 0u;
 #pragma unroll
-  for (int i = 0; i < R; ++i) {
-    float v[VEC];
-    V::get(raw[i], v);
-    top = quant_top(v, top);
-  }
-  top = quant_lanes_top(top, kWave);
+  for (int i = 0; i < R; ++i) top = V::top(raw[i], top);
+  top = quant_lanes_top(V::bits(top), kWave);
   if constexpr (NT > kWave) {
     if (lane_id() == 0) tops[threadIdx.x >> 6] = top;
     __syncthreads();
@@ -202,7 +220,7 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void quant_row_kernel(const Qu
     const int at = tid + i * NT;
     if (at < a.nv) {
       float v[VEC];
-      int n[VEC];
+      unsigned n[VEC];
       V::get(raw[i], v);
       qr.integers(v, n);
       quant_store(q + (long)at * VEC, n);
@@ -217,12 +235,8 @@ __global__ __launch_bounds__(1024) void quant_long_kernel(const QuantArgs a) {
   __shared__ unsigned tops[16];
   const T* const x = (const T*)a.x + (long)blockIdx.x * a.ldx;
   unsigned top = 0u;
-  for (int at = (int)threadIdx.x; at < a.nv; at += 1024) {
-    float v[VEC];
-    V::get(ld((const typename V::raw*)(x + (long)at * VEC)), v);
-    top = quant_top(v, top);
-  }
-  top = quant_lanes_top(top, kWave);
+  for (int at = (int)threadIdx.x; at < a.nv; at += 1024) top = V::top(ld((const typename V::raw*)(x + (long)at * VEC)), top);
+  top = quant_lanes_top(V::bits(top), kWave);
   if (lane_id() == 0) tops[threadIdx.x >> 6] = top;
   __syncthreads();
 #pragma unroll
@@ -231,7 +245,7 @@ __global__ __launch_bounds__(1024) void quant_long_kernel(const QuantArgs a) {
   if (threadIdx.x == 0) st(a.scale + (long)blockIdx.x, qr.scale);
   for (int at = (int)threadIdx.x; at < a.nv; at += 1024) {
     float v[VEC];
-    int n[VEC];
+    unsigned n[VEC];
     V::get(ld((const typename V::raw*)(x + (long)at * VEC)), v);
     qr.integers(v, n);
     quant_store(a.q + (long)blockIdx.x * a.ldq + (long)at * VEC, n);

@@ -322,28 +322,33 @@ __device__ __forceinline__ uint4 i8_chunk(const signed char* row, int at, int k)
   return q;
 }
 // ---- few tokens (m <= 32): bound by the weights' bytes ----------------------------------------------------------------------
-// A workgroup takes 16 output channels; its eight waves share the sum in units of 128 bytes.  Weights go from memory straight into
-// the matrix instruction's registers (16 rows x 64 bytes each), the tokens' bytes come from the caches in the same order of k,
-// and the waves' partial sums meet in LDS: one launch, no workspace.  Four units (eight 16-byte loads a lane) are in flight per
-// wave.
+// A workgroup takes 16 NT output channels; its eight waves share the sum in units of 128 bytes.  Weights go from memory straight
+// into the matrix instruction's registers (16 rows x 64 bytes each), the tokens' bytes come from the caches in the same order of
+// k, and the waves' partial sums meet in LDS: one launch, no workspace.  Four units of loads are in flight per wave.
+// Every workgroup reads all tokens: NT = 2 halves that where the channels still give half of the compute units a workgroup
+// (32 tokens, 5120 x 4096 weights: the tokens' 42 MB through the L2s cost more than the 21 MB of weights from memory).
 constexpr int kTokWaves = 8, kTokUnit = 128, kTokFlight = 4;
-template <int MT, bool FAST, typename T>
+template <int NT, int MT, bool FAST, typename T>
 __global__ __launch_bounds__(512) void i8_token_kernel(const I8Args a) {
-  __shared__ i32x4 red[kTokWaves][MT][kWave];
+  __shared__ i32x4 red[kTokWaves][NT * MT][kWave];
   const int lane = lane_id(), wave = uniform((int)(threadIdx.x >> 6));
-  const int n0 = (int)blockIdx.x * 16;
+  const int n0 = (int)blockIdx.x * 16 * NT;
   const int r16 = lane & 15, kc = (lane >> 4) * 16;
   // (channels and tokens behind the last: the last one's bytes, their outputs are not stored)
-  const signed char* wrow = a.w + (long)(n0 + r16 < a.n ? n0 + r16 : a.n - 1) * a.ldw;
+  const signed char* wrow[NT];
   const signed char* xrow[MT];
 #pragma unroll
-  for (int t = 0; t < MT; ++t) xrow[t] = a.x + (t * 16 + r16 < a.m ? t * 16 + r16 : a.m - 1) * a.ldx;
-  i32x4 acc[MT];
+  for (int c = 0; c < NT; ++c) wrow[c] = a.w + (long)(n0 + c * 16 + r16 < a.n ? n0 + c * 16 + r16 : a.n - 1) * a.ldw;
 #pragma unroll
-  for (int t = 0; t < MT; ++t) acc[t] = i32x4{0, 0, 0, 0};
+  for (int t = 0; t < MT; ++t) xrow[t] = a.x + (t * 16 + r16 < a.m ? t * 16 + r16 : a.m - 1) * a.ldx;
+  i32x4 acc[NT][MT];
+#pragma unroll
+  for (int c = 0; c < NT; ++c)
+#pragma unroll
+    for (int t = 0; t < MT; ++t) acc[c][t] = i32x4{0, 0, 0, 0};
   const int units = (a.k + kTokUnit - 1) / kTokUnit;
   for (int u0 = wave; u0 < units; u0 += kTokWaves * kTokFlight) {
-    uint4 wq[kTokFlight][2], xq[kTokFlight][2][MT];
+    uint4 wq[kTokFlight][2][NT], xq[kTokFlight][2][MT];
 #pragma unroll
     for (int f = 0; f < kTokFlight; ++f)
 #pragma unroll
@@ -352,11 +357,13 @@ __global__ __launch_bounds__(512) void i8_token_kernel(const I8Args a) {
         if constexpr (FAST) {
           // every load is issued: behind the end the row's last chunk again, with the weights zeroed
           const int from = at < a.k ? at : a.k - 16;
-          wq[f][h] = ld((const uint4*)(wrow + from));
+#pragma unroll
+          for (int c = 0; c < NT; ++c) wq[f][h][c] = ld((const uint4*)(wrow[c] + from));
 #pragma unroll
           for (int t = 0; t < MT; ++t) xq[f][h][t] = ld((const uint4*)(xrow[t] + from));
         } else {
-          wq[f][h] = i8_chunk(wrow, at, a.k);
+#pragma unroll
+          for (int c = 0; c < NT; ++c) wq[f][h][c] = i8_chunk(wrow[c], at, a.k);
 #pragma unroll
           for (int t = 0; t < MT; ++t) xq[f][h][t] = i8_chunk(xrow[t], at, a.k);
         }
@@ -366,26 +373,32 @@ __global__ __launch_bounds__(512) void i8_token_kernel(const I8Args a) {
       for (int f = 0; f < kTokFlight; ++f)
 #pragma unroll
         for (int h = 0; h < 2; ++h)
-          if ((u0 + f * kTokWaves) * kTokUnit + h * 64 + kc >= a.k) wq[f][h] = make_uint4(0u, 0u, 0u, 0u);
+          if ((u0 + f * kTokWaves) * kTokUnit + h * 64 + kc >= a.k) {
+#pragma unroll
+            for (int c = 0; c < NT; ++c) wq[f][h][c] = make_uint4(0u, 0u, 0u, 0u);
+          }
     }
 #pragma unroll
     for (int f = 0; f < kTokFlight; ++f)
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int t = 0; t < MT; ++t) acc[t] = mfma_16x16x64_i8(wq[f][h], xq[f][h][t], acc[t]);
+        for (int c = 0; c < NT; ++c)
+#pragma unroll
+          for (int t = 0; t < MT; ++t) acc[c][t] = mfma_16x16x64_i8(wq[f][h][c], xq[f][h][t], acc[c][t]);
   }
 #pragma unroll
-  for (int t = 0; t < MT; ++t) red[wave][t][lane] = acc[t];
+  for (int c = 0; c < NT; ++c)
+#pragma unroll
+    for (int t = 0; t < MT; ++t) red[wave][c * MT + t][lane] = acc[c][t];
   __syncthreads();
-  const int tid = (int)threadIdx.x;
-  if (tid < MT * 256) {       // one output each: channel fastest
-    const int t = tid >> 8, tok = (tid >> 4) & 15, ch = tid & 15;
-    const int from = (ch >> 2) * 16 + tok;
+  for (int o = (int)threadIdx.x; o < NT * MT * 256; o += kTokWaves * kWave) {       // one output each: channel fastest
+    const int ch = o % (16 * NT), tok = o / (16 * NT);
+    const int tile = (ch >> 4) * MT + (tok >> 4), from = ((ch & 15) >> 2) * 16 + (tok & 15);
     int sum = 0;
 #pragma unroll
-    for (int v = 0; v < kTokWaves; ++v) sum += red[v][t][from][ch & 3];
-    const int i = t * 16 + tok, j = n0 + ch;
+    for (int v = 0; v < kTokWaves; ++v) sum += red[v][tile][from][ch & 3];
+    const int i = tok, j = n0 + ch;
     if (i < a.m && j < a.n)
       i8_store((T*)a.y + (long)i * a.ldy + j,
                i8_epilogue(sum, ld(a.sx + i), ld(a.sw + j), a.bias ? ld(a.bias + j) : 0.0f, a.act));
@@ -768,13 +781,23 @@ static int i8_launch_tile(I8Args& a, int num_cu, hipStream_t st) {
 template <typename T>
 static int i8_launch(const eco_inner_product_i8_plan& p, I8Args& a, bool fast, hipStream_t st) {
   if (a.m <= kTokMax) {
-    const dim3 grid((unsigned)ceil_div(a.n, 16)), block(kTokWaves * kWave);
+    const dim3 grid((unsigned)ceil_div(a.n, p.bn)), block(kTokWaves * kWave);
     if (a.m <= 16) {
-      if (fast) hipLaunchKernelGGL((i8_token_kernel<1, true, T>), grid, block, 0, st, a);
-      else hipLaunchKernelGGL((i8_token_kernel<1, false, T>), grid, block, 0, st, a);
+      if (p.bn == 32) {
+        if (fast) hipLaunchKernelGGL((i8_token_kernel<2, 1, true, T>), grid, block, 0, st, a);
+        else hipLaunchKernelGGL((i8_token_kernel<2, 1, false, T>), grid, block, 0, st, a);
+      } else {
+        if (fast) hipLaunchKernelGGL((i8_token_kernel<1, 1, true, T>), grid, block, 0, st, a);
+        else hipLaunchKernelGGL((i8_token_kernel<1, 1, false, T>), grid, block, 0, st, a);
+      }
     } else {
-      if (fast) hipLaunchKernelGGL((i8_token_kernel<2, true, T>), grid, block, 0, st, a);
-      else hipLaunchKernelGGL((i8_token_kernel<2, false, T>), grid, block, 0, st, a);
+      if (p.bn == 32) {
+        if (fast) hipLaunchKernelGGL((i8_token_kernel<2, 2, true, T>), grid, block, 0, st, a);
+        else hipLaunchKernelGGL((i8_token_kernel<2, 2, false, T>), grid, block, 0, st, a);
+      } else {
+        if (fast) hipLaunchKernelGGL((i8_token_kernel<1, 2, true, T>), grid, block, 0, st, a);
+        else hipLaunchKernelGGL((i8_token_kernel<1, 2, false, T>), grid, block, 0, st, a);
+      }
     }
     return check_launch("eco_inner_product_i8_forward(tokens)");
   }
@@ -829,7 +852,7 @@ extern "C" int eco_inner_product_i8_plan_create(int64_t m, int64_t n, int64_t k,
   plan->m = m; plan->n = (int32_t)n; plan->k = (int32_t)k; plan->dt = dt;
   plan->num_cu = num_cu ? num_cu : current_device_num_cu();
   if (m <= kTokMax) {
-    plan->bm = m <= 16 ? 16 : 32; plan->bn = 16; plan->ksplit = 1;
+    plan->bm = m <= 16 ? 16 : 32; plan->bn = m > 4 && ceil_div(n, 32) >= plan->num_cu / 2 ? 32 : 16; plan->ksplit = 1;
     return ECO_OK;
   }
   // The tile with the least time by a model in cycles of a compute unit: rounds of tiles x (stages x cost of a stage + cost of

@@ -321,15 +321,17 @@ __device__ __forceinline__ uint4 i8_chunk(const signed char* row, int at, int k)
   }
   return q;
 }
-// ---- few tokens (m <= 32): bound by the weights' bytes ----------------------------------------------------------------------
+// ---- few tokens (m <= 64): bound by the weights' bytes ----------------------------------------------------------------------
 // A workgroup takes 16 NT output channels; its eight waves share the sum in units of 128 bytes.  Weights go from memory straight
 // into the matrix instruction's registers (16 rows x 64 bytes each), the tokens' bytes come from the caches in the same order of
-// k, and the waves' partial sums meet in LDS: one launch, no workspace.  Four units of loads are in flight per wave.
+// k, and the waves' partial sums meet in LDS: one launch, no workspace.  Four units of loads are in flight per wave (two of 64
+// tokens).
 // Every workgroup reads all tokens: NT = 2 halves that where the channels still give half of the compute units a workgroup
 // (32 tokens, 5120 x 4096 weights: the tokens' 42 MB through the L2s cost more than the 21 MB of weights from memory).
-constexpr int kTokWaves = 8, kTokUnit = 128, kTokFlight = 4;
+constexpr int kTokWaves = 8, kTokUnit = 128;
 template <int NT, int MT, bool FAST, typename T>
 __global__ __launch_bounds__(512) void i8_token_kernel(const I8Args a) {
+  constexpr int kTokFlight = MT > 2 ? 2 : 4;
   __shared__ i32x4 red[kTokWaves][NT * MT][kWave];
   const int lane = lane_id(), wave = uniform((int)(threadIdx.x >> 6));
   const int n0 = (int)blockIdx.x * 16 * NT;
@@ -420,7 +422,7 @@ __global__ __launch_bounds__(512) void i8_token_kernel(const I8Args a) {
 //         fragments -- is refilled.  A tile's scales and bias come the same way, into one of three slots.
 //   else  any alignment: one tile a workgroup, operands through registers
 template <int B, int NBUF, bool FAST, typename T>
-__global__ __launch_bounds__(256, B > 128 ? 1 : 3) void i8_tile_kernel(const I8Args a) {
+__global__ __launch_bounds__(256, B > 128 || NBUF == 6 ? 1 : NBUF == 8 ? 2 : 3) void i8_tile_kernel(const I8Args a) {
   constexpr int W = B / 2, TW = W / 16;                  // TW x TW products of 16x16 a wave
   constexpr bool BIG = B > 128;                          // (taken with whole sums and 16-byte stores only)
   constexpr int STAGE = 2 * B * 4;                       // 16-byte vectors of a stage: B rows of w, then B rows of x
@@ -436,9 +438,10 @@ __global__ __launch_bounds__(256, B > 128 ? 1 : 3) void i8_tile_kernel(const I8A
   // Tile numbers: XCD b % 8 owns a contiguous range, its workgroups take every gx-th of it; inside, groups of eight row tiles
   // by all channel tiles: the tiles that run side by side on an XCD share their operands through its L2.
   const int tiles = a.tiles_m * a.tiles_n, total = tiles * a.ksplit;
-  const int xcd = (int)blockIdx.x & 7, gx = ((int)gridDim.x - xcd + 7) >> 3;
-  const int xbase = xcd * (total >> 3) + (xcd < (total & 7) ? xcd : (total & 7));
-  const int xend = xbase + (total >> 3) + (xcd < (total & 7) ? 1 : 0);
+  const int xcds = (int)gridDim.x < 8 ? (int)gridDim.x : 8;         // (a launch of fewer workgroups: each a range of its own)
+  const int xcd = (int)blockIdx.x % xcds, place = (int)blockIdx.x / xcds, gx = ((int)gridDim.x - xcd + xcds - 1) / xcds;
+  const int each = total / xcds, more = total - each * xcds;
+  const int xbase = xcd * each + (xcd < more ? xcd : more), xend = xbase + each + (xcd < more ? 1 : 0);
   struct Item {
     long m0;
     int n0, slice, s_begin, s_end, ns;
@@ -570,7 +573,7 @@ __global__ __launch_bounds__(256, B > 128 ? 1 : 3) void i8_tile_kernel(const I8A
   };
 
   clear();
-  int id = xbase + ((int)blockIdx.x >> 3);
+  int id = xbase + place;
   Item cur = item_of(id);
 
   if constexpr (FAST) {
@@ -758,7 +761,7 @@ static inline unsigned i8_grid(long count, long per_block) {
   return (unsigned)(g > 1048576 ? 1048576 : g);   // grid-stride beyond this
 }
 
-constexpr int kTokMax = 32;     // rows up to which the token kernel is taken
+constexpr int kTokMax = 64;     // rows up to which the token kernel is taken
 
 template <int B, int NBUF, bool FAST, typename T>
 static int i8_launch_tile(I8Args& a, int num_cu, hipStream_t st) {
@@ -766,7 +769,7 @@ static int i8_launch_tile(I8Args& a, int num_cu, hipStream_t st) {
   a.tiles_n = (int)ceil_div(a.n, B);
   const long total = (long)a.tiles_m * a.tiles_n * a.ksplit;
   constexpr int kLds = NBUF * 2 * B * 64 + 3 * 3 * B * 4;
-  constexpr int kPerCu = B > 128 ? 1 : B > 64 ? 3 : 6;     // workgroups that a compute unit's 160 KB of LDS hold
+  constexpr int kPerCu = B > 128 || NBUF == 6 ? 1 : NBUF == 8 ? 2 : B > 64 ? 3 : 6;   // workgroups that a compute unit's 160 KB of LDS hold
   const long grid = FAST && B <= 128 && total > (long)kPerCu * num_cu ? (long)kPerCu * num_cu : total;
   ECO_RAISE_DYNAMIC_LDS((i8_tile_kernel<B, NBUF, FAST, T>), "inner_product_i8");
   hipLaunchKernelGGL((i8_tile_kernel<B, NBUF, FAST, T>), dim3((unsigned)grid), dim3(kI8Threads), (unsigned)kLds, st, a);
@@ -778,33 +781,27 @@ static int i8_launch_tile(I8Args& a, int num_cu, hipStream_t st) {
   return ECO_OK;
 }
 
+template <int NT, int MT, typename T>
+static int i8_launch_tokens(const I8Args& a, bool fast, hipStream_t st) {
+  const dim3 grid((unsigned)ceil_div(a.n, 16 * NT)), block(kTokWaves * kWave);
+  if (fast) hipLaunchKernelGGL((i8_token_kernel<NT, MT, true, T>), grid, block, 0, st, a);
+  else hipLaunchKernelGGL((i8_token_kernel<NT, MT, false, T>), grid, block, 0, st, a);
+  return check_launch("eco_inner_product_i8_forward(tokens)");
+}
+
 template <typename T>
 static int i8_launch(const eco_inner_product_i8_plan& p, I8Args& a, bool fast, hipStream_t st) {
   if (a.m <= kTokMax) {
-    const dim3 grid((unsigned)ceil_div(a.n, p.bn)), block(kTokWaves * kWave);
-    if (a.m <= 16) {
-      if (p.bn == 32) {
-        if (fast) hipLaunchKernelGGL((i8_token_kernel<2, 1, true, T>), grid, block, 0, st, a);
-        else hipLaunchKernelGGL((i8_token_kernel<2, 1, false, T>), grid, block, 0, st, a);
-      } else {
-        if (fast) hipLaunchKernelGGL((i8_token_kernel<1, 1, true, T>), grid, block, 0, st, a);
-        else hipLaunchKernelGGL((i8_token_kernel<1, 1, false, T>), grid, block, 0, st, a);
-      }
-    } else {
-      if (p.bn == 32) {
-        if (fast) hipLaunchKernelGGL((i8_token_kernel<2, 2, true, T>), grid, block, 0, st, a);
-        else hipLaunchKernelGGL((i8_token_kernel<2, 2, false, T>), grid, block, 0, st, a);
-      } else {
-        if (fast) hipLaunchKernelGGL((i8_token_kernel<1, 2, true, T>), grid, block, 0, st, a);
-        else hipLaunchKernelGGL((i8_token_kernel<1, 2, false, T>), grid, block, 0, st, a);
-      }
-    }
-    return check_launch("eco_inner_product_i8_forward(tokens)");
+    if (p.bn == 32) return a.m <= 16 ? i8_launch_tokens<2, 1, T>(a, fast, st) : a.m <= 32 ? i8_launch_tokens<2, 2, T>(a, fast, st) : i8_launch_tokens<2, 4, T>(a, fast, st);
+    return a.m <= 16 ? i8_launch_tokens<1, 1, T>(a, fast, st) : a.m <= 32 ? i8_launch_tokens<1, 2, T>(a, fast, st) : i8_launch_tokens<1, 4, T>(a, fast, st);
   }
   if (fast) {
     if (p.bm == 256 && a.vec) return i8_launch_tile<256, 4, true, T>(a, p.num_cu, st);
-    if (p.bm >= 128) return i8_launch_tile<128, 3, true, T>(a, p.num_cu, st);
-    return i8_launch_tile<64, 3, true, T>(a, p.num_cu, st);
+    // Where a compute unit gets one 128 tile or two 64 tiles at most, nothing but more stages ahead hides the loads: the buffers
+    // take the LDS that more workgroups would (1024 x 4096 x 4096: 26.5 us with three buffers, 20 with six).
+    const long tiles = ceil_div(a.m, p.bm) * ceil_div(a.n, p.bm) * a.ksplit;
+    if (p.bm >= 128) return p.bm == 128 && tiles <= p.num_cu ? i8_launch_tile<128, 6, true, T>(a, p.num_cu, st) : i8_launch_tile<128, 3, true, T>(a, p.num_cu, st);
+    return tiles <= 2l * p.num_cu ? i8_launch_tile<64, 8, true, T>(a, p.num_cu, st) : i8_launch_tile<64, 3, true, T>(a, p.num_cu, st);
   }
   if (p.bm >= 128) return i8_launch_tile<128, 2, false, T>(a, p.num_cu, st);
   return i8_launch_tile<64, 2, false, T>(a, p.num_cu, st);
@@ -852,31 +849,36 @@ extern "C" int eco_inner_product_i8_plan_create(int64_t m, int64_t n, int64_t k,
   plan->m = m; plan->n = (int32_t)n; plan->k = (int32_t)k; plan->dt = dt;
   plan->num_cu = num_cu ? num_cu : current_device_num_cu();
   if (m <= kTokMax) {
-    plan->bm = m <= 16 ? 16 : 32; plan->bn = m > 4 && ceil_div(n, 32) >= plan->num_cu / 2 ? 32 : 16; plan->ksplit = 1;
+    plan->bm = m <= 16 ? 16 : m <= 32 ? 32 : 64; plan->bn = m > 4 && ceil_div(n, 32) >= plan->num_cu / 2 ? 32 : 16; plan->ksplit = 1;
     return ECO_OK;
   }
-  // The tile with the least time by a model in cycles of a compute unit: rounds of tiles x (stages x cost of a stage + cost of
-  // a tile's start and end).  A stage of 64 bytes costs a 256 x 256 tile its products (1024 cycles, the LDS three quarters
-  // busy), smaller tiles their LDS traffic (48 and 24 KB at 128 bytes a cycle); starts and ends hide behind the
-  // neighbours that the smaller tiles' LDS leaves room for.
-  const long cu = plan->num_cu, stages = ceil_div(k, 64);
-  const auto tiles = [&](long bm, long bn) { return ceil_div(m, bm) * ceil_div(n, bn); };
-  const auto cost = [&](long b, long stage, long ends) { return ceil_div(tiles(b, b), cu) * (stages * stage + ends); };
-  const long c256 = cost(256, 1300, 8000), c128 = cost(128, 420, 2000), c64 = cost(64, 210, 900);
-  const bool big = n % 8 == 0 && c256 <= c128 && c256 <= c64;      // (its stores are 16 bytes wide)
-  plan->bm = plan->bn = big ? 256 : c128 <= c64 ? 128 : 64;
-  plan->ksplit = 1;
-  const long t = tiles(plan->bm, plan->bn);
-  ECO_REQUIRE(t <= 2147483647l / 16, "inner_product_i8: too many tiles for one launch");
-  if (!big && t < cu && stages >= 16) {     // too few tiles: cut long sums so that two workgroups a compute unit run, of eight stages at least
-    long ks = ceil_div(2 * cu, t);
-    if (ks > stages / 8) ks = stages / 8;
-    if (ks > 16) ks = 16;
-    if (ks > 1) {
-      plan->ksplit = (int32_t)ks;
-      plan->ws_bytes = ks * m * n * 4;
+  // The tile and the cut with the least time by a model in cycles of a compute unit.  A compute unit's share of the tiles costs
+  // stages x cost of a stage + cost of a tile's start and end: a stage of 64 bytes costs a 256 x 256 tile its products (1024 cycles,
+  // the LDS half busy), smaller tiles their LDS traffic, and no stage less than its loads' way (150 cycles with the deep buffers).
+  // All tiles' operands pass the L2s at about 2.6 KB a cycle.  A cut sum's parts are written and read at 2 KB a cycle, by one launch
+  // more.
+  const double cu = plan->num_cu, stages = (double)ceil_div(k, 64);
+  double least = 0.0;
+  for (int b = 64; b <= 256; b *= 2)
+    for (int ks = 1; ks <= 16; ks *= 2) {
+      if (b == 256 && (ks > 1 || n % 8)) continue;              // (its stores are 16 bytes wide)
+      if (ks > 1 && stages < 4 * ks) continue;                  // four stages of a slice at least
+      const double tiles = (double)ceil_div(m, b) * (double)ceil_div(n, b) * ks, per = stages / ks;
+      if (ks > 1 && tiles > 4 * cu) continue;
+      const double stage = b == 256 ? 1300 : b == 128 ? 420 : 210, ends = b == 256 ? 8000 : b == 128 ? 2500 : 1200;
+      const double share = (double)(int64_t)((tiles + cu - 1) / cu);
+      double t = share * (per * stage + ends);
+      const double l2 = tiles * per * b * 128 / 2600;
+      t = (t > l2 ? t : l2) + 3000;
+      if (ks > 1) t += 7000 + (double)m * (double)n * ks * 8 / 2000;
+      if (least == 0.0 || t < least) {
+        least = t;
+        plan->bm = plan->bn = b;
+        plan->ksplit = ks;
+      }
     }
-  }
+  ECO_REQUIRE(ceil_div(m, plan->bm) * ceil_div(n, plan->bn) <= 2147483647l / 16, "inner_product_i8: too many tiles for one launch");
+  if (plan->ksplit > 1) plan->ws_bytes = (int64_t)plan->ksplit * m * n * 4;
   return ECO_OK;
 }
 

@@ -193,7 +193,8 @@ def test_product_strides_alignment_and_guards(backend, m, dt, gaps, shifts):
 
 
 @pytest.mark.parametrize("num_cu", [1, 5])
-@pytest.mark.parametrize("m,n,k", [(5, 24, 700), (90, 50, 640), (300, 260, 70)])
+@pytest.mark.parametrize("m,n,k", [(5, 24, 700), (20, 40, 352), (40, 70, 288), (64, 33, 100), (90, 50, 640), (90, 56, 1040), (300, 260, 70), (200, 200, 512),
+                                   (600, 520, 96)])
 def test_product_plans_for_other_sizes_of_device(backend, m, n, k, num_cu):
     run_product(backend, m, n, k, hip.DT_F32, num_cu=num_cu, act=hip.ACT_SILU)
 

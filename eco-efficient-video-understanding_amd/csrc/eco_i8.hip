@@ -287,7 +287,7 @@ struct I8Args {
   long m;
   int n, k, act;
   int vec;                 // y's rows allow 16-byte stores of eight (f32: four) consecutive channels
-  int ksplit, nstages;     // slices; 64-byte stages of the whole sum
+  int ksplit, nstages;     // slices; 128-byte stages of the whole sum
   int tiles_m, tiles_n;
 };
 
@@ -411,23 +411,28 @@ __global__ __launch_bounds__(512) void i8_token_kernel(const I8Args a) {
 // A workgroup of four waves takes B output channels x B rows, each wave W x W of them (W = B / 2) as 16x16 products over 64 bytes
 // of k (D's rows are channels, so that a lane ends up with consecutive channels of one row of y).  16x16x64 rather than
 // 32x32x32: the same rate, half the accumulator traffic a product -- and this kernel runs at the clock that its power allows.
-// Both operands pass through LDS in stages of 64 bytes of k, rows 64 bytes apart, the four 16-byte chunks of row r stored in
-// the order c ^ (-(r >> 2) & 3): the sixteen lanes that a fragment's 16-byte read serves at once (0-3, 12-15, 20-23, 24-27,
-// then the others) touch all 64 banks once.  A wave holds a stage's
-// fragments in registers, twice: the next stage's are read while this one's products run.
+// Both operands pass through LDS in stages of 128 bytes of k -- whole cache lines: with rows of 64 bytes every line was asked of
+// the L2 twice, and the requests, not the bytes, were its limit --, rows 128 bytes apart, the eight 16-byte chunks of row r
+// stored in the order c ^ ((r >> 1) & 7): the sixteen lanes that a fragment's 16-byte read serves at once (0-3, 12-15, 20-23,
+// 24-27, then the others) touch all 64 banks once.  A wave holds the fragments of half a stage in registers, twice: the next
+// half's are read while this one's products run.
 //   FAST  (rows on 16-byte boundaries, k a multiple of 16): persistent workgroups walk their tiles' stages as ONE stream through
 //         NBUF buffers filled by LDS-DMA -- across the ends of tiles, so that a tile's stores run under the next one's loads.
 //         (The 256 tile's sums fill the accumulator file, fragments held across its end would spill: one tile a workgroup.)
-//         One barrier a stage: behind it the next stage has landed, and the buffer of this one -- every wave has its
-//         fragments -- is refilled.  A tile's scales and bias come the same way, into one of three slots.
+//         One barrier in the middle of a stage: behind it the next stage has landed, and the buffer of this one -- every wave
+//         has its last fragments -- is refilled.  A tile's scales and bias come the same way, into one of NBUF + 2
+//         slots (a tile of one stage: asked for when the tile NBUF before it is still unfinished, one ahead of its stage).
 //   else  any alignment: one tile a workgroup, operands through registers
+// Workgroups that a compute unit's 160 KB of LDS hold.
+constexpr int i8_tile_lds(int b, int nbuf) { return nbuf * 2 * b * 128 + (nbuf + 2) * 3 * b * 4; }
+constexpr int i8_tile_per_cu(int b, int nbuf) { return 160 * 1024 / i8_tile_lds(b, nbuf); }
 template <int B, int NBUF, bool FAST, typename T>
-__global__ __launch_bounds__(256, B > 128 || NBUF == 6 ? 1 : NBUF == 8 ? 2 : 3) void i8_tile_kernel(const I8Args a) {
+__global__ __launch_bounds__(256, i8_tile_per_cu(B, NBUF)) void i8_tile_kernel(const I8Args a) {
   constexpr int W = B / 2, TW = W / 16;                  // TW x TW products of 16x16 a wave
   constexpr bool BIG = B > 128;                          // (taken with whole sums and 16-byte stores only)
-  constexpr int STAGE = 2 * B * 4;                       // 16-byte vectors of a stage: B rows of w, then B rows of x
-  constexpr int NR = 2 * TW, NP = TW * TW;               // fragments and products of a stage
-  constexpr int PW = B / 64;                             // DMA pieces (16 rows x 64 bytes) of a wave per stage and operand
+  constexpr int STAGE = 2 * B * 8;                       // 16-byte vectors of a stage: B rows of w, then B rows of x
+  constexpr int NR = 2 * TW, NP = TW * TW;               // fragments and products of half a stage
+  constexpr int PW = B / 32;                             // DMA pieces (8 rows x 128 bytes) of a wave per stage and operand
   constexpr int SLOT = 3 * B;                            // floats of a tile's parameters: sw, bias, sx
   ECO_DYNAMIC_LDS(lds_f);
   uint4* const lds = (uint4*)lds_f;
@@ -444,7 +449,7 @@ __global__ __launch_bounds__(256, B > 128 || NBUF == 6 ? 1 : NBUF == 8 ? 2 : 3) 
   const int xbase = xcd * each + (xcd < more ? xcd : more), xend = xbase + each + (xcd < more ? 1 : 0);
   struct Item {
     long m0;
-    int n0, slice, s_begin, s_end, ns;
+    int n0, slice, s_begin, ns;
   };
   auto item_of = [&](int id) {
     Item t;
@@ -456,10 +461,8 @@ __global__ __launch_bounds__(256, B > 128 || NBUF == 6 ? 1 : NBUF == 8 ? 2 : 3) 
     t.m0 = (long)uniform(8 * grp + in - q * gm) * B;
     t.n0 = uniform(q * B);
     t.slice = uniform(t.slice);
-    t.s_begin = uniform(a.nstages * t.slice / a.ksplit);              // (at most 2048 stages, 16 slices)
-    // (an even number of stages, for the two fragment sets; a stage behind the slice's end is zeros)
-    t.s_end = uniform(a.nstages * (t.slice + 1) / a.ksplit);
-    t.ns = (t.s_end - t.s_begin + 1) & ~1;
+    t.s_begin = uniform(a.nstages * t.slice / a.ksplit);              // (at most 1024 stages, 16 slices of one at least)
+    t.ns = uniform(a.nstages * (t.slice + 1) / a.ksplit) - t.s_begin;
     return t;
   };
 
@@ -471,12 +474,12 @@ __global__ __launch_bounds__(256, B > 128 || NBUF == 6 ? 1 : NBUF == 8 ? 2 : 3) 
       for (int j = 0; j < TW; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
   };
   uint4 wf[2][TW], xf[2][TW];
-  // fragment r of a stage (r < TW: w's, else x's)
-  const int fk = (lane >> 4) ^ (-(lane >> 2) & 3);
-  const int fw = (wn + (lane & 15)) * 4 + fk, fx = (B + wm + (lane & 15)) * 4 + fk;
-  auto read_frag = [&](int slot, const uint4* buf, int r) {
-    if (r < TW) wf[slot][r] = buf[fw + 64 * r];
-    else xf[slot][r - TW] = buf[fx + 64 * (r - TW)];
+  // fragment r of half `h` of a stage (r < TW: w's, else x's)
+  const int fk[2] = {(lane >> 4) ^ ((lane & 15) >> 1), (4 + (lane >> 4)) ^ ((lane & 15) >> 1)};
+  const int fw = (wn + (lane & 15)) * 8, fx = (B + wm + (lane & 15)) * 8;
+  auto read_frag = [&](int h, const uint4* buf, int r) {
+    if (r < TW) wf[h][r] = buf[fw + fk[h] + 128 * r];
+    else xf[h][r - TW] = buf[fx + fk[h] + 128 * (r - TW)];
   };
 
   // A lane holds row m0 + wm + 16 j + (lane & 15) and channels 4 (lane >> 4) + {0..3} of each 16-channel block.
@@ -577,9 +580,9 @@ __global__ __launch_bounds__(256, B > 128 || NBUF == 6 ? 1 : NBUF == 8 ? 2 : 3) 
   Item cur = item_of(id);
 
   if constexpr (FAST) {
-    const int prow = lane >> 2, pchunk = (lane & 3) ^ (-(prow >> 2) & 3);
+    const int prow = lane >> 3, pchunk = (lane & 7) ^ ((wave & 1) * 4 + (prow >> 1));
     const unsigned vw = (unsigned)((long)prow * a.ldw + pchunk * 16), vx = (unsigned)((long)prow * a.ldx + pchunk * 16);
-    const unsigned ldw16 = (unsigned)(16 * a.ldw), ldx16 = (unsigned)(16 * a.ldx);
+    const unsigned ldw8 = (unsigned)(8 * a.ldw), ldx8 = (unsigned)(8 * a.ldx);
     // ---- the asking side of the stream: item, stage in it, its operands' descriptors (from the tile's first row to the
     // operand's end: rows behind the last one read zeros) ----
     Item ask = cur;
@@ -598,7 +601,7 @@ __global__ __launch_bounds__(256, B > 128 || NBUF == 6 ? 1 : NBUF == 8 ? 2 : 3) 
 #ifndef ECO_EMU
         asm volatile("s_nop 4" ::"s"(rp));
 #endif
-        if (lane < B / 4) glds16_buf(rp, (unsigned)lane * 16u, 0u, (uint4*)(params + (ask_tile % 3) * SLOT + wave * B));
+        if (lane < B / 4) glds16_buf(rp, (unsigned)lane * 16u, 0u, (uint4*)(params + (ask_tile % (NBUF + 2)) * SLOT + wave * B));
       }
 #ifndef ECO_EMU
       // (descriptor words written by readfirstlane: five wait states before a memory instruction inside asm may read them)
@@ -608,12 +611,12 @@ __global__ __launch_bounds__(256, B > 128 || NBUF == 6 ? 1 : NBUF == 8 ? 2 : 3) 
     // piece p (0 .. 2 PW - 1: w's, then x's) of the stage that is asked for next
     auto ask_piece = [&](int p, unsigned k0, unsigned off) {
       uint4* const buf = lds + (asked % NBUF) * STAGE;
-      if (p < PW) glds16_buf(rw, off, k0 + (unsigned)(p * 4 + wave) * ldw16, buf + (p * 4 + wave) * 64);
-      else glds16_buf(rx, off, k0 + (unsigned)((p - PW) * 4 + wave) * ldx16, buf + B * 4 + ((p - PW) * 4 + wave) * 64);
+      if (p < PW) glds16_buf(rw, off, k0 + (unsigned)(p * 4 + wave) * ldw8, buf + (p * 4 + wave) * 64);
+      else glds16_buf(rx, off, k0 + (unsigned)((p - PW) * 4 + wave) * ldx8, buf + B * 8 + ((p - PW) * 4 + wave) * 64);
     };
-    auto ask_k0 = [&]() { return (unsigned)((ask.s_begin + ask_s) * 64); };
+    auto ask_k0 = [&]() { return (unsigned)((ask.s_begin + ask_s) * 128); };
     // (chunks behind k, and the stages asked for behind the stream's end: zeros, nothing is read)
-    auto ask_in_k = [&]() { return ask_more && ask.s_begin + ask_s < ask.s_end && (int)ask_k0() + pchunk * 16 < a.k; };
+    auto ask_in_k = [&]() { return ask_more && (int)ask_k0() + pchunk * 16 < a.k; };
     auto ask_next = [&]() {             // one stage further
       ++asked;
       if (++ask_s == ask.ns && ask_more) {
@@ -627,36 +630,31 @@ __global__ __launch_bounds__(256, B > 128 || NBUF == 6 ? 1 : NBUF == 8 ? 2 : 3) 
         }
       }
     };
-    // One stage: the products of fragment set `slot`, and between them, in the first three quarters, the other set's fragments
-    // are read from buffer `buf` (the last quarter is the time they have to arrive) and, evenly spaced -- the address unit
-    // takes 16 cycles for a piece, and all four waves ask at once --, the pieces of the next asked stage go out: the
+    // Half a stage: the products of its fragments, and between them, in the first three quarters, the other half's fragments are
+    // read from buffer `buf` (the last quarter is the time they have to arrive); in the second half, evenly spaced, the pieces
+    // of the next asked stage go out -- the address unit takes 16 cycles for a piece, and all four waves ask at once.  The
     // matrix unit works on meanwhile.
-    auto stage = [&](auto slot_c, auto last_c, const uint4* buf) {
-      constexpr int slot = decltype(slot_c)::value;
-      constexpr bool last = decltype(last_c)::value;       // products only
+    auto half_stage = [&](auto half_c, const uint4* buf) {
+      constexpr int h = decltype(half_c)::value;
       const unsigned k0 = ask_k0(), ow = ask_in_k() ? vw : kBufOob, ox = ask_in_k() ? vx : kBufOob;
       static_for<NP>([&](auto qc) {
         constexpr int q = decltype(qc)::value, i = q / TW, j = q % TW;
-        if constexpr (BIG) mfma_16x16x64_i8_agpr(acc[i][j], wf[slot][i], xf[slot][j]);
-        else acc[i][j] = mfma_16x16x64_i8(wf[slot][i], xf[slot][j], acc[i][j]);
-        if constexpr (!last) {
-          constexpr int r0 = 4 * q * NR / (3 * NP) < NR ? 4 * q * NR / (3 * NP) : NR;
-          constexpr int r1 = 4 * (q + 1) * NR / (3 * NP) < NR ? 4 * (q + 1) * NR / (3 * NP) : NR;
-          constexpr int p0 = q * 2 * PW / NP, p1 = (q + 1) * 2 * PW / NP;
-          if constexpr (r1 > r0 || p1 > p0) sched_fence();
+        if constexpr (BIG) mfma_16x16x64_i8_agpr(acc[i][j], wf[h][i], xf[h][j]);
+        else acc[i][j] = mfma_16x16x64_i8(wf[h][i], xf[h][j], acc[i][j]);
+        constexpr int r0 = 4 * q * NR / (3 * NP) < NR ? 4 * q * NR / (3 * NP) : NR;
+        constexpr int r1 = 4 * (q + 1) * NR / (3 * NP) < NR ? 4 * (q + 1) * NR / (3 * NP) : NR;
+        constexpr int p0 = h ? q * 2 * PW / NP : 0, p1 = h ? (q + 1) * 2 * PW / NP : 0;
+        if constexpr (r1 > r0 || p1 > p0) sched_fence();
 #pragma unroll
-          for (int r = r0; r < r1; ++r) read_frag(slot ^ 1, buf, r);
+        for (int r = r0; r < r1; ++r) read_frag(h ^ 1, buf, r);
 #pragma unroll
-          for (int p = p0; p < p1; ++p) ask_piece(p, k0, p < PW ? ow : ox);
-          if constexpr (r1 > r0 || p1 > p0) sched_fence();
-        }
+        for (int p = p0; p < p1; ++p) ask_piece(p, k0, p < PW ? ow : ox);
+        if constexpr (r1 > r0 || p1 > p0) sched_fence();
       });
-      if constexpr (!last) ask_next();
+      if constexpr (h) ask_next();
     };
     constexpr std::integral_constant<int, 0> c0{};
     constexpr std::integral_constant<int, 1> c1{};
-    constexpr std::false_type no{};
-    constexpr std::true_type yes{};
 
     if constexpr (BIG) agpr_sums_settled();
     describe();
@@ -671,22 +669,17 @@ __global__ __launch_bounds__(256, B > 128 || NBUF == 6 ? 1 : NBUF == 8 ? 2 : 3) 
 #pragma unroll
     for (int r = 0; r < NR; ++r) read_frag(0, lds, r);
     int g = 0;                          // stages taken
-    // behind it: every wave has its fragments of stage g, and stage g + 1 -- of g + 1 .. g + NBUF - 1 in flight -- has landed
-    // (stores and parameter pieces among the newer operations only make the wait stricter)
-    auto turn = [&]() {
-      wait_lds_reads();
-      wait_dma_all_but<(NBUF - 2) * 2 * PW>();
-      wg_barrier_nodrain();
-      ++g;
-    };
     for (int tile = 0;; ++tile) {
-      for (int s = 0; s < cur.ns; s += 2) {
-        turn();
-        stage(c0, no, lds + (g % NBUF) * STAGE);
-        turn();
-        stage(c1, no, lds + (g % NBUF) * STAGE);
+      for (int s = 0; s < cur.ns; ++s, ++g) {
+        half_stage(c0, lds + (g % NBUF) * STAGE);
+        // every wave has its last fragments of stage g, and stage g + 1 -- of g + 1 .. g + NBUF - 1 in flight -- has landed
+        // (stores and parameter pieces among the newer operations only make the wait stricter)
+        wait_lds_reads();
+        wait_dma_all_but<(NBUF - 2) * 2 * PW>();
+        wg_barrier_nodrain();
+        half_stage(c1, lds + ((g + 1) % NBUF) * STAGE);
       }
-      finish(cur, params + (tile % 3) * SLOT);
+      finish(cur, params + (tile % (NBUF + 2)) * SLOT);
       if constexpr (BIG) break;         // (one tile a workgroup)
       id += gx;
       if (id >= xend) break;
@@ -701,42 +694,43 @@ __global__ __launch_bounds__(256, B > 128 || NBUF == 6 ? 1 : NBUF == 8 ? 2 : 3) 
       params[B + c] = a.bias ? ld(a.bias + ch) : 0.0f;
       params[2 * B + c] = ld(a.sx + (cur.m0 + c < a.m ? cur.m0 + c : a.m - 1));
     }
-    constexpr int CH = STAGE / 256;       // chunks of a thread per stage
-    constexpr int AHEAD = B > 64 ? 2 : 4;   // stages in registers
+    constexpr int CH = STAGE / 256, AHEAD = 2;       // chunks of a thread per stage, stages in registers
     uint4 q[AHEAD][CH];
-    const int ns = cur.s_end - cur.s_begin;
     auto fetch = [&](int s, uint4 (&to)[CH]) {
-      const int k0 = (cur.s_begin + s) * 64;
+      const int k0 = (cur.s_begin + s) * 128;
 #pragma unroll
       for (int p = 0; p < CH; ++p) {
-        const int id4 = p * 256 + tid, row = id4 >> 2, at = k0 + (id4 & 3) * 16;
+        const int c = p * 256 + tid, row = c >> 3, at = k0 + (c & 7) * 16;
         to[p] = make_uint4(0u, 0u, 0u, 0u);
         if (row < B) { if (cur.n0 + row < a.n) to[p] = i8_chunk(a.w + (long)(cur.n0 + row) * a.ldw, at, a.k); }
         else if (cur.m0 + row - B < a.m) to[p] = i8_chunk(a.x + (cur.m0 + row - B) * a.ldx, at, a.k);
       }
     };
-    static_for<AHEAD>([&](auto d) { if (decltype(d)::value < ns) fetch(decltype(d)::value, q[decltype(d)::value]); });
-    for (int s0 = 0; s0 < ns; s0 += AHEAD)
+    static_for<AHEAD>([&](auto d) { if (decltype(d)::value < cur.ns) fetch(decltype(d)::value, q[decltype(d)::value]); });
+    for (int s0 = 0; s0 < cur.ns; s0 += AHEAD)
       static_for<AHEAD>([&](auto d) {
         constexpr int v = decltype(d)::value;
         const int s = s0 + v;
-        if (s < ns) {
+        if (s < cur.ns) {
           uint4* const buf = lds + (s & 1) * STAGE;
 #pragma unroll
           for (int p = 0; p < CH; ++p) {
-            const int id4 = p * 256 + tid, row = id4 >> 2;
-            buf[row * 4 + ((id4 & 3) ^ (-(row >> 2) & 3))] = q[v][p];
+            const int c = p * 256 + tid, row = c >> 3;
+            buf[row * 8 + ((c & 7) ^ ((row >> 1) & 7))] = q[v][p];
           }
-          if (s + AHEAD < ns) fetch(s + AHEAD, q[v]);
+          if (s + AHEAD < cur.ns) fetch(s + AHEAD, q[v]);
           // (one barrier a stage: a wave may write buffer s+1 -- last read in stage s-1 -- while others still read buffer s)
           wait_lds_reads();
           wg_barrier_nodrain();
 #pragma unroll
-          for (int r = 0; r < NR; ++r) read_frag(0, buf, r);
+          for (int h = 0; h < 2; ++h) {
 #pragma unroll
-          for (int i = 0; i < TW; ++i)
+            for (int r = 0; r < NR; ++r) read_frag(h, buf, r);
 #pragma unroll
-            for (int j = 0; j < TW; ++j) acc[i][j] = mfma_16x16x64_i8(wf[0][i], xf[0][j], acc[i][j]);
+            for (int i = 0; i < TW; ++i)
+#pragma unroll
+              for (int j = 0; j < TW; ++j) acc[i][j] = mfma_16x16x64_i8(wf[h][i], xf[h][j], acc[i][j]);
+          }
         }
       });
     finish(cur, params);
@@ -768,8 +762,7 @@ static int i8_launch_tile(I8Args& a, int num_cu, hipStream_t st) {
   a.tiles_m = (int)ceil_div(a.m, B);
   a.tiles_n = (int)ceil_div(a.n, B);
   const long total = (long)a.tiles_m * a.tiles_n * a.ksplit;
-  constexpr int kLds = NBUF * 2 * B * 64 + 3 * 3 * B * 4;
-  constexpr int kPerCu = B > 128 || NBUF == 6 ? 1 : NBUF == 8 ? 2 : B > 64 ? 3 : 6;   // workgroups that a compute unit's 160 KB of LDS hold
+  constexpr int kLds = i8_tile_lds(B, NBUF), kPerCu = i8_tile_per_cu(B, NBUF);
   const long grid = FAST && B <= 128 && total > (long)kPerCu * num_cu ? (long)kPerCu * num_cu : total;
   ECO_RAISE_DYNAMIC_LDS((i8_tile_kernel<B, NBUF, FAST, T>), "inner_product_i8");
   hipLaunchKernelGGL((i8_tile_kernel<B, NBUF, FAST, T>), dim3((unsigned)grid), dim3(kI8Threads), (unsigned)kLds, st, a);
@@ -795,16 +788,14 @@ static int i8_launch(const eco_inner_product_i8_plan& p, I8Args& a, bool fast, h
     if (p.bn == 32) return a.m <= 16 ? i8_launch_tokens<2, 1, T>(a, fast, st) : a.m <= 32 ? i8_launch_tokens<2, 2, T>(a, fast, st) : i8_launch_tokens<2, 4, T>(a, fast, st);
     return a.m <= 16 ? i8_launch_tokens<1, 1, T>(a, fast, st) : a.m <= 32 ? i8_launch_tokens<1, 2, T>(a, fast, st) : i8_launch_tokens<1, 4, T>(a, fast, st);
   }
-  if (fast) {
-    if (p.bm == 256 && a.vec) return i8_launch_tile<256, 4, true, T>(a, p.num_cu, st);
-    // Where a compute unit gets one 128 tile or two 64 tiles at most, nothing but more stages ahead hides the loads: the buffers
-    // take the LDS that more workgroups would (1024 x 4096 x 4096: 26.5 us with three buffers, 20 with six).
-    const long tiles = ceil_div(a.m, p.bm) * ceil_div(a.n, p.bm) * a.ksplit;
-    if (p.bm >= 128) return p.bm == 128 && tiles <= p.num_cu ? i8_launch_tile<128, 6, true, T>(a, p.num_cu, st) : i8_launch_tile<128, 3, true, T>(a, p.num_cu, st);
-    return tiles <= 2l * p.num_cu ? i8_launch_tile<64, 8, true, T>(a, p.num_cu, st) : i8_launch_tile<64, 3, true, T>(a, p.num_cu, st);
-  }
-  if (p.bm >= 128) return i8_launch_tile<128, 2, false, T>(a, p.num_cu, st);
-  return i8_launch_tile<64, 2, false, T>(a, p.num_cu, st);
+  if (!fast) return i8_launch_tile<64, 2, false, T>(a, p.num_cu, st);
+  if (p.bm == 256 && a.vec) return i8_launch_tile<256, 2, true, T>(a, p.num_cu, st);
+  // Where a compute unit gets one 128 tile or two 64 tiles at most, nothing but more stages ahead hides the loads: the buffers
+  // take the LDS that more workgroups would.
+  const int b = p.bm >= 128 ? 128 : 64;
+  const long tiles = ceil_div(a.m, b) * ceil_div(a.n, b) * a.ksplit;
+  if (b == 128) return tiles <= p.num_cu ? i8_launch_tile<128, 4, true, T>(a, p.num_cu, st) : i8_launch_tile<128, 2, true, T>(a, p.num_cu, st);
+  return tiles <= 2l * p.num_cu ? i8_launch_tile<64, 4, true, T>(a, p.num_cu, st) : i8_launch_tile<64, 2, true, T>(a, p.num_cu, st);
 }
 
 }  // namespace eco
@@ -862,7 +853,7 @@ extern "C" int eco_inner_product_i8_plan_create(int64_t m, int64_t n, int64_t k,
   for (int b = 64; b <= 256; b *= 2)
     for (int ks = 1; ks <= 16; ks *= 2) {
       if (b == 256 && (ks > 1 || n % 8)) continue;              // (its stores are 16 bytes wide)
-      if (ks > 1 && stages < 4 * ks) continue;                  // four stages of a slice at least
+      if (ks > 1 && stages < 4 * ks) continue;                  // 256 bytes of a slice at least
       const double tiles = (double)ceil_div(m, b) * (double)ceil_div(n, b) * ks, per = stages / ks;
       if (ks > 1 && tiles > 4 * cu) continue;
       const double stage = b == 256 ? 1300 : b == 128 ? 420 : 210, ends = b == 256 ? 8000 : b == 128 ? 2500 : 1200;
@@ -908,7 +899,7 @@ extern "C" int eco_inner_product_i8_forward(const eco_inner_product_i8_plan* pla
   const size_t es = plan->dt == ECO_DT_F32 ? 4 : 2;
   a.vec = a.n % 8 == 0 && (uintptr_t)y % 16 == 0 && (a.ldy * es) % 16 == 0;
   a.ksplit = plan->ksplit;
-  a.nstages = (int)ceil_div(a.k, 64);
+  a.nstages = (int)ceil_div(a.k, 128);
   // 16-byte chunks of either operand inside its rows and on 16-byte boundaries; a tile's rows within the descriptors' 2 GB
   const bool fast = a.k % 16 == 0 && a.ldx % 16 == 0 && a.ldw % 16 == 0 && ((uintptr_t)x | (uintptr_t)w) % 16 == 0 &&
                     256 * a.ldx + a.k < 0x7fffffffl && 256 * a.ldw + a.k < 0x7fffffffl;

@@ -303,24 +303,41 @@ __device__ __forceinline__ float i8_epilogue(int acc, float sx, float sw, float 
 __device__ __forceinline__ void i8_store(float* p, float v) { st(p, v); }
 __device__ __forceinline__ void i8_store(unsigned short* p, float v) { st(p, (unsigned short)f32_to_bf16_bits(v)); }
 
-// Sixteen bytes of a row from byte `at` on (at < k): an unaligned 16-byte load, or -- where the row ends inside -- its last bytes
-// one by one and zeros.  Nothing outside the row is read.
+// Sixteen bytes of a row from byte `at` on: an unaligned 16-byte load, or -- where the row ends inside -- its last bytes one by one
+// and zeros.  Nothing outside the row is read.  (Explicitly global: through a pointer that the compiler takes for a generic one
+// the loads count as LDS operations too, and every wait for LDS waits for them.)
 __device__ __forceinline__ uint4 i8_chunk(const signed char* row, int at, int k) {
   uint4 q = make_uint4(0u, 0u, 0u, 0u);
-  if (at + 16 <= k) {
 #ifdef ECO_EMU
-    if (!emu::check_access(row + at, 16, false)) return q;
-#endif
-    __builtin_memcpy(&q, row + at, 16);
+  const signed char* g = row;
+  if (at + 16 <= k) {
+    if (emu::check_access(row + at, 16, false)) memcpy(&q, row + at, 16);
   } else if (at < k) {
+#else
+  typedef const __attribute__((address_space(1))) signed char* global_bytes;
+  typedef unsigned u32x4_u __attribute__((ext_vector_type(4), aligned(1)));
+  const global_bytes g = (global_bytes)row;
+  if (at + 16 <= k) {
+    const u32x4_u v = *(const __attribute__((address_space(1))) u32x4_u*)(g + at);
+    q = make_uint4(v.x, v.y, v.z, v.w);
+  } else if (at < k) {
+#endif
     unsigned u[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
     for (int e = 0; e < 16; ++e)
-      if (at + e < k) u[e >> 2] |= (unsigned)(unsigned char)ld(row + at + e) << (8 * (e & 3));
+      if (at + e < k) {
+#ifdef ECO_EMU
+        const unsigned char v = (unsigned char)ld(g + at + e);
+#else
+        const unsigned char v = (unsigned char)g[at + e];
+#endif
+        u[e >> 2] |= (unsigned)v << (8 * (e & 3));
+      }
     q = make_uint4(u[0], u[1], u[2], u[3]);
   }
   return q;
 }
+
 // ---- few tokens (m <= 64): bound by the weights' bytes ----------------------------------------------------------------------
 // A workgroup takes 16 NT output channels; its eight waves share the sum in units of 128 bytes.  Weights go from memory straight
 // into the matrix instruction's registers (16 rows x 64 bytes each), the tokens' bytes come from the caches in the same order of
@@ -700,10 +717,10 @@ __global__ __launch_bounds__(256, i8_tile_per_cu(B, NBUF)) void i8_tile_kernel(c
       const int k0 = (cur.s_begin + s) * 128;
 #pragma unroll
       for (int p = 0; p < CH; ++p) {
-        const int c = p * 256 + tid, row = c >> 3, at = k0 + (c & 7) * 16;
-        to[p] = make_uint4(0u, 0u, 0u, 0u);
-        if (row < B) { if (cur.n0 + row < a.n) to[p] = i8_chunk(a.w + (long)(cur.n0 + row) * a.ldw, at, a.k); }
-        else if (cur.m0 + row - B < a.m) to[p] = i8_chunk(a.x + (cur.m0 + row - B) * a.ldx, at, a.k);
+        // (rows behind the last: the last one's bytes, their sums are not stored)
+        const int row = (p % (CH / 2)) * 32 + (tid >> 3), at = k0 + (tid & 7) * 16;
+        if (p < CH / 2) to[p] = i8_chunk(a.w + (long)(cur.n0 + row < a.n ? cur.n0 + row : a.n - 1) * a.ldw, at, a.k);
+        else to[p] = i8_chunk(a.x + (cur.m0 + row < a.m ? cur.m0 + row : a.m - 1) * a.ldx, at, a.k);
       }
     };
     static_for<AHEAD>([&](auto d) { if (decltype(d)::value < cur.ns) fetch(decltype(d)::value, q[decltype(d)::value]); });
@@ -843,25 +860,22 @@ extern "C" int eco_inner_product_i8_plan_create(int64_t m, int64_t n, int64_t k,
     plan->bm = m <= 16 ? 16 : m <= 32 ? 32 : 64; plan->bn = m > 4 && ceil_div(n, 32) >= plan->num_cu / 2 ? 32 : 16; plan->ksplit = 1;
     return ECO_OK;
   }
-  // The tile and the cut with the least time by a model in cycles of a compute unit.  A compute unit's share of the tiles costs
-  // stages x cost of a stage + cost of a tile's start and end: a stage of 64 bytes costs a 256 x 256 tile its products (1024 cycles,
-  // the LDS half busy), smaller tiles their LDS traffic, and no stage less than its loads' way (150 cycles with the deep buffers).
-  // All tiles' operands pass the L2s at about 2.6 KB a cycle.  A cut sum's parts are written and read at 2 KB a cycle, by one launch
-  // more.
-  const double cu = plan->num_cu, stages = (double)ceil_div(k, 64);
+  // The tile and the cut with the least time by a model in microseconds, fitted to sweeps of both over 20 sizes (100 x 1024 x 1024
+  // to 401408 x 64 x 192) on 256 compute units: rounds x (stages x time of a stage + a tile's start and end).  Tiles of 64 and 128 run
+  // several to a compute unit, so rounds count in parts, but one alone waits for its loads (1.15 and 1.45 rounds at least).  A cut sum
+  // costs a launch and its parts' way through memory at 2 TB/s: worth it where tiles are few and sums long (65 x 512 x 8192:
+  // 18.0 us whole, 10.8 in eight; 128 x 8192 x 8192: 20.0 whole, 25.3 in two).
+  const double cu = plan->num_cu, stages = (double)ceil_div(k, 128);
   double least = 0.0;
   for (int b = 64; b <= 256; b *= 2)
     for (int ks = 1; ks <= 16; ks *= 2) {
       if (b == 256 && (ks > 1 || n % 8)) continue;              // (its stores are 16 bytes wide)
-      if (ks > 1 && stages < 4 * ks) continue;                  // 256 bytes of a slice at least
-      const double tiles = (double)ceil_div(m, b) * (double)ceil_div(n, b) * ks, per = stages / ks;
-      if (ks > 1 && tiles > 4 * cu) continue;
-      const double stage = b == 256 ? 1300 : b == 128 ? 420 : 210, ends = b == 256 ? 8000 : b == 128 ? 2500 : 1200;
-      const double share = (double)(int64_t)((tiles + cu - 1) / cu);
-      double t = share * (per * stage + ends);
-      const double l2 = tiles * per * b * 128 / 2600;
-      t = (t > l2 ? t : l2) + 3000;
-      if (ks > 1) t += 7000 + (double)m * (double)n * ks * 8 / 2000;
+      if (ks > 1 && stages < 2 * ks) continue;
+      const double rounds = (double)ceil_div(m, b) * (double)ceil_div(n, b) * ks / cu, per = stages / ks;
+      double t = b == 64    ? (rounds > 1.15 ? rounds : 1.15) * (0.19 * per + 0.5)
+                 : b == 128 ? (rounds > 1.45 ? rounds : 1.45) * (0.49 * per + 1.2)
+                            : ceil(rounds) * (1.62 * per + 6.0);
+      if (ks > 1) t += 4.0 + (double)m * (double)n * ks * 8.0 / 2e6;
       if (least == 0.0 || t < least) {
         least = t;
         plan->bm = plan->bn = b;

@@ -576,9 +576,10 @@ extern "C" int eco_group_norm_plan_create(int64_t n, int64_t s, int32_t c, int32
   ECO_REQUIRE(plan != nullptr, "group_norm: null plan");
   ECO_REQUIRE(n >= 0 && s >= 0, "group_norm: negative shape");
   ECO_REQUIRE(c > 0 && groups > 0 && c % groups == 0, "group_norm: %d groups do not divide %d channels", groups, c);
+  ECO_REQUIRE(c <= (1 << 30), "group_norm: too many channels");
   ECO_REQUIRE(dt == ECO_DT_F32 || dt == ECO_DT_BF16, "group_norm: unknown type %d", dt);
   ECO_REQUIRE(num_cu >= 0, "group_norm: negative num_cu");
-  ECO_REQUIRE(s <= 2147483647l && n <= 2147483647l / groups, "group_norm: too many positions or images for one launch");
+  ECO_REQUIRE(s <= (1l << 30) && n <= 2147483647l / groups, "group_norm: too many positions or images for one launch");
   memset(plan, 0, sizeof(*plan));
   plan->n = n; plan->s = s; plan->c = c; plan->groups = groups; plan->dt = dt;
   plan->num_cu = num_cu ? num_cu : current_device_num_cu();

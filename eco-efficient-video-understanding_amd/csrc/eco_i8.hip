@@ -778,7 +778,8 @@ template <int B, int NBUF, bool FAST, typename T>
 static int i8_launch_tile(I8Args& a, int num_cu, hipStream_t st) {
   a.tiles_m = (int)ceil_div(a.m, B);
   a.tiles_n = (int)ceil_div(a.n, B);
-  const long total = (long)a.tiles_m * a.tiles_n * a.ksplit;
+  const long total = ceil_div(a.m, B) * ceil_div(a.n, B) * a.ksplit;
+  ECO_REQUIRE(total <= 2147483647l, "inner_product_i8: too many tiles for one launch");
   constexpr int kLds = i8_tile_lds(B, NBUF), kPerCu = i8_tile_per_cu(B, NBUF);
   const long grid = FAST && B <= 128 && total > (long)kPerCu * num_cu ? (long)kPerCu * num_cu : total;
   ECO_RAISE_DYNAMIC_LDS((i8_tile_kernel<B, NBUF, FAST, T>), "inner_product_i8");
@@ -824,7 +825,7 @@ extern "C" int eco_quant_rows_forward(const void* x, int32_t dt, int64_t ldx, in
   clear_error();
   ECO_REQUIRE(dt == ECO_DT_F32 || dt == ECO_DT_BF16, "quant_rows: unknown type %d", dt);
   ECO_REQUIRE(m >= 0 && k > 0, "quant_rows: bad shape");
-  ECO_REQUIRE(m <= 2147483647l && k <= 2147483647l, "quant_rows: too many rows or columns");
+  ECO_REQUIRE(m <= 2147483647l && k <= (1l << 30), "quant_rows: too many rows or columns");
   if (m == 0) return ECO_OK;
   ECO_REQUIRE(x && q && scale, "quant_rows: null argument");
   const size_t es = dt == ECO_DT_F32 ? 4 : 2;
@@ -850,7 +851,7 @@ extern "C" int eco_inner_product_i8_plan_create(int64_t m, int64_t n, int64_t k,
   ECO_REQUIRE(plan != nullptr, "inner_product_i8: null plan");
   ECO_REQUIRE(m >= 0 && n > 0 && k > 0, "inner_product_i8: bad shape");
   ECO_REQUIRE(k <= ECO_I8_MAX_K, "inner_product_i8: sums of %ld products can leave 32 bits (at most %d)", (long)k, ECO_I8_MAX_K);
-  ECO_REQUIRE(m <= 2147483647l && n <= 2147483647l, "inner_product_i8: too many rows");
+  ECO_REQUIRE(m <= 2147483647l && n <= (1l << 30), "inner_product_i8: too many rows or channels");
   ECO_REQUIRE(dt == ECO_DT_F32 || dt == ECO_DT_BF16, "inner_product_i8: unknown type %d", dt);
   ECO_REQUIRE(num_cu >= 0, "inner_product_i8: negative num_cu");
   memset(plan, 0, sizeof(*plan));
@@ -882,7 +883,7 @@ extern "C" int eco_inner_product_i8_plan_create(int64_t m, int64_t n, int64_t k,
         plan->ksplit = ks;
       }
     }
-  ECO_REQUIRE(ceil_div(m, plan->bm) * ceil_div(n, plan->bn) <= 2147483647l / 16, "inner_product_i8: too many tiles for one launch");
+  ECO_REQUIRE(ceil_div(m, 64) * ceil_div(n, 64) * plan->ksplit <= 2147483647l, "inner_product_i8: too many tiles for one launch");
   if (plan->ksplit > 1) plan->ws_bytes = (int64_t)plan->ksplit * m * n * 4;
   return ECO_OK;
 }

@@ -136,6 +136,8 @@ SHAPES = [  # n, s, c, groups
     (1, 200, 48, 3), (1, 9, 512, 32), (1, 5, 2600, 13), (2, 3, 4104, 2), (1, 700, 8, 2), (5, 64, 12, 12), (1, 40, 260, 130),
     # more channels than a workgroup's threads take at once, groups across its tiles
     (2, 90, 4104, 2), (1, 150, 2600, 13), (1, 70, 2049, 1), (1, 130, 1030, 103), (1, 1500, 48, 4),
+    # images that no workgroup's registers hold
+    (3, 700, 96, 1), (2, 1100, 64, 1), (1, 2100, 256, 256), (1, 9000, 16, 1), (1, 11000, 6, 1), (1, 33000, 1, 1), (2, 4500, 32, 2),
 ]
 
 
@@ -158,7 +160,7 @@ def test_plans_for_other_sizes_of_device(backend, dt, num_cu):
 
 
 @pytest.mark.parametrize("dt", [hip.DT_F32, hip.DT_BF16], ids=["f32", "bf16"])
-@pytest.mark.parametrize("shape", [(6, 37, 64, 8), (6, 37, 30, 3), (6, 400, 16, 4)], ids=lambda v: "x".join(map(str, v)))
+@pytest.mark.parametrize("shape", [(6, 37, 64, 8), (6, 37, 30, 3), (6, 400, 16, 4), (6, 700, 96, 1), (6, 1100, 64, 1), (6, 90, 2600, 2)], ids=lambda v: "x".join(map(str, v)))
 def test_lengths(backend, dt, shape):
     """From none to all, one beyond either end; what lies behind a length is NaN and must not be seen."""
     s = shape[1]
@@ -177,10 +179,11 @@ def test_lengths(backend, dt, shape):
 def test_strides_alignment_and_guards(backend, dt, row_gap, image_gap, shift, in_place):
     run(backend, 3, 21, 48, 6, dt, row_gap=row_gap, image_gap=image_gap, shift=shift, in_place=in_place, act=hip.ACT_RELU)
     run(backend, 2, 600, 16, 2, dt, row_gap=row_gap, image_gap=image_gap, shift=shift, in_place=in_place)
+    run(backend, 2, 700, 96, 1, dt, row_gap=row_gap, image_gap=image_gap, shift=shift, in_place=in_place, lengths=[650, 3])
 
 
 @pytest.mark.parametrize("dt", [hip.DT_F32, hip.DT_BF16], ids=["f32", "bf16"])
-@pytest.mark.parametrize("s", [20, 900])
+@pytest.mark.parametrize("s", [20, 900, 5000])
 def test_nan_and_infinity_stay_in_their_group(backend, dt, s):
     x = values(np.random.default_rng(8), 3, s, 32, dt)
     x[0, s // 2, 5] = np.nan
@@ -191,7 +194,7 @@ def test_nan_and_infinity_stay_in_their_group(backend, dt, s):
     case.check()
 
 
-@pytest.mark.parametrize("s", [15, 1000])
+@pytest.mark.parametrize("s", [15, 1000, 6000])
 def test_values_far_from_zero(backend, s):
     """A mean of a hundred spreads; a first position far from all others; a constant group (its variance is 0)."""
     x = values(np.random.default_rng(9), 2, s, 24, hip.DT_F32) + 100.0
@@ -202,6 +205,15 @@ def test_values_far_from_zero(backend, s):
     case.check()
 
 
+def test_all_lengths_zero(backend):
+    """Nothing of x is read and nothing of y written (both images of it, in either form)."""
+    for s, c, g in ((12, 16, 4), (700, 96, 1)):
+        x = np.full((3, s, c), np.nan, np.float32)
+        case = Case(backend, 3, s, c, g, hip.DT_F32, lengths=[0, 0, -1], x=x)
+        case.call()
+        case.check()
+
+
 def test_nothing_to_do(backend):
     for n, s in ((0, 5), (5, 0), (0, 0)):
         p = backend.lib.group_norm_plan(n, s, 8, 2, hip.DT_F32)
@@ -209,7 +221,7 @@ def test_nothing_to_do(backend):
 
 
 REFUSED_PLANS = [dict(n=-1), dict(s=-1), dict(c=0), dict(groups=0), dict(groups=3), dict(groups=16), dict(dt=2), dict(num_cu=-1),
-                 dict(n=2 ** 40), dict(s=2 ** 40)]
+                 dict(n=2 ** 40), dict(s=2 ** 40), dict(s=2 ** 30 + 1), dict(c=2 ** 30 + 2)]
 
 
 @pytest.mark.parametrize("kw", REFUSED_PLANS, ids=lambda v: "-".join(f"{a}{b}" for a, b in v.items()))

@@ -107,7 +107,7 @@ def test_quant_nothing_to_do_and_refusals(backend):
     p = backend.alloc.ptr
     ok = dict(x=p(x), dt=hip.DT_F32, q=p(q), scale=p(s), m=4, k=8)
     for kw in (dict(dt=2), dict(m=-1), dict(k=0), dict(x=None), dict(q=None), dict(scale=None), dict(ldx=7), dict(ldq=7),
-               dict(ldx=-8), dict(x=p(x) + 2), dict(ldx=2 ** 62), dict(ldq=2 ** 62), dict(k=2 ** 40)):
+               dict(ldx=-8), dict(x=p(x) + 2), dict(ldx=2 ** 62), dict(ldq=2 ** 62), dict(k=2 ** 40), dict(k=2 ** 30 + 1, ldx=2 ** 31), dict(m=2 ** 31)):
         with pytest.raises(hip.EcoError, match="quant_rows"):
             lib.quant_rows_forward(**{**ok, **kw})
     assert (backend.host(q, (64,)) == 99).all() and (backend.host(s, (8,)) == 5.0).all()
@@ -124,7 +124,7 @@ def operand(be, a, gap, shift, fill=113):
 
 class Product:
     def __init__(self, be, m, n, k, dt, act=hip.ACT_NONE, bias=True, gaps=(0, 0, 0), shifts=(0, 0, 0), seed=0, num_cu=None,
-                 extreme=False):
+                 extreme=False, scale_shift=0):
         rng = np.random.default_rng(seed)
         self.be, self.m, self.n, self.k, self.dt, self.act, self.gaps, self.shifts = be, m, n, k, dt, act, gaps, shifts
         if extreme:
@@ -136,8 +136,11 @@ class Product:
         self.bias = rng.standard_normal(n).astype(np.float32) if bias else None
         self.plan = be.lib.inner_product_i8_plan(m, n, k, dt, num_cu)
         self.dx, self.dw = operand(be, self.x, gaps[0], shifts[0]), operand(be, self.w, gaps[1], shifts[1])
-        self.dsx, self.dsw = be.dev(self.sx), be.dev(self.sw)
-        self.db = be.dev(self.bias) if bias else None
+        # scales and bias `scale_shift` floats into their buffers: on a 4-byte boundary, no more
+        self.scale_shift = scale_shift
+        lead = np.full(scale_shift, 7.0, np.float32)
+        self.dsx, self.dsw = be.dev(np.concatenate([lead, self.sx])), be.dev(np.concatenate([lead, self.sw]))
+        self.db = be.dev(np.concatenate([lead, self.bias])) if bias else None
         self.total = shifts[2] + m * (n + gaps[2])
         self.dy = be.dev(store(np.full(self.total, 3.0, np.float32), dt))
         self.ws = be.empty((self.plan.ws_bytes // 4,), np.int32) if self.plan.ws_bytes else None
@@ -147,8 +150,10 @@ class Product:
         size = 4 if self.dt == hip.DT_F32 else 2
         args = dict(act=self.act, ldx=self.k + self.gaps[0], ldw=self.k + self.gaps[1], ldy=self.n + self.gaps[2], workspace=p(self.ws))
         args.update(kw)
-        self.be.lib.inner_product_i8_forward(self.plan, p(self.dx) + self.shifts[0], p(self.dsx), p(self.dw) + self.shifts[1],
-                                             p(self.dsw), p(self.db), p(self.dy) + self.shifts[2] * size, **args)
+        f = 4 * self.scale_shift
+        self.be.lib.inner_product_i8_forward(self.plan, p(self.dx) + self.shifts[0], p(self.dsx) + f, p(self.dw) + self.shifts[1],
+                                             p(self.dsw) + f, p(self.db) + f if self.db is not None else None,
+                                             p(self.dy) + self.shifts[2] * size, **args)
 
     def check(self):
         flat = value(self.be.host(self.dy, (self.total,)), self.dt)
@@ -192,6 +197,12 @@ def test_product_strides_alignment_and_guards(backend, m, dt, gaps, shifts):
     run_product(backend, m, 37, 83, dt, gaps=gaps, shifts=shifts, bias=False)
 
 
+@TYPES
+@pytest.mark.parametrize("m,n,k,shift", [(3, 40, 64, 1), (70, 72, 96, 1), (200, 136, 160, 3), (300, 264, 64, 2), (90, 37, 50, 1)])
+def test_product_scales_on_any_boundary(backend, m, n, k, shift, dt):
+    run_product(backend, m, n, k, dt, scale_shift=shift, act=hip.ACT_SILU)
+
+
 @pytest.mark.parametrize("num_cu", [1, 5])
 @pytest.mark.parametrize("m,n,k", [(5, 24, 700), (20, 40, 352), (40, 70, 288), (64, 33, 100), (90, 50, 640), (90, 56, 1040), (300, 260, 70), (200, 200, 512),
                                    (600, 520, 96)])
@@ -220,7 +231,7 @@ def test_product_nothing_to_do(backend):
     backend.lib.inner_product_i8_forward(p, None, None, None, None, None, None)
 
 
-@pytest.mark.parametrize("kw", [dict(m=-1), dict(n=0), dict(k=0), dict(k=hip.I8_MAX_K + 1), dict(m=2 ** 31), dict(n=2 ** 31), dict(dt=2),
+@pytest.mark.parametrize("kw", [dict(m=-1), dict(n=0), dict(k=0), dict(k=hip.I8_MAX_K + 1), dict(m=2 ** 31), dict(n=2 ** 31), dict(n=2 ** 30 + 1), dict(m=2 ** 31 - 1, n=2 ** 30), dict(dt=2),
                                 dict(num_cu=-1)], ids=lambda v: "-".join(f"{a}{b}" for a, b in v.items()))
 def test_product_refused_plans(backend, kw):
     with pytest.raises(hip.EcoError, match="inner_product_i8"):

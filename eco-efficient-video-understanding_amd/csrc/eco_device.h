@@ -20,7 +20,6 @@
 #include <utility>
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef int i32x16 __attribute__((ext_vector_type(16)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 namespace eco {
@@ -50,17 +49,9 @@ __device__ __forceinline__ f32x16 mfma_32x32x16_bf16(uint4 a, uint4 b, f32x16 c)
 #endif
 }
 
-// D(32x32) += A(32x32) * B(32x32), int8 in / int32 accumulate (v_mfma_i32_32x32x32_i8): lane l supplies sixteen consecutive k of
-// row / column l&31, A[l&31][16*(l>>5) + e]; C/D as the f32 form.  Any permutation of k that A and B share gives the same sum.
-__device__ __forceinline__ i32x16 mfma_32x32x32_i8(uint4 a, uint4 b, i32x16 c) {
-#ifdef ECO_EMU
-  return emu::mfma_i32_32x32x32_i8(a, b, c);
-#else
-  return __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b), c, 0, 0, 0);
-#endif
-}
-// D(16x16) += A(16x64) * B(64x16) (v_mfma_i32_16x16x64_i8): lane l supplies A[l&15][16*(l>>4) + e]; reg r of the result is
-// D[4*(l>>4) + r][l&15].
+// D(16x16) += A(16x64) * B(64x16), int8 in / int32 accumulate (v_mfma_i32_16x16x64_i8): lane l supplies sixteen consecutive k of row /
+// column l&15, A[l&15][16*(l>>4) + e]; reg r of the result is D[4*(l>>4) + r][l&15].  Any permutation of k that A and B share
+// gives the same sum.
 __device__ __forceinline__ i32x4 mfma_16x16x64_i8(uint4 a, uint4 b, i32x4 c) {
 #ifdef ECO_EMU
   return emu::mfma_i32_16x16x64_i8(a, b, c);
@@ -370,7 +361,7 @@ __device__ __forceinline__ float shfl_xor(float v, int mask) {
 }
 
 // v / (1 + exp(-v)) on the hardware's 2^x and reciprocal (one unit in the last place each): off by at most (7 + |v|) * 2^-24
-// relative; 0 below v = -89, where the value is under 2^-120.
+// relative down to v = -87; 0 below v = -87.4, where the reciprocal leaves fp32's normal range and the value is under 1e-36.
 __device__ __forceinline__ float silu(float v) {
 #ifdef ECO_EMU
   return v * (1.0f / (1.0f + exp2f(v * -1.44269504f)));

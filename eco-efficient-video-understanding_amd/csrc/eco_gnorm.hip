@@ -537,12 +537,21 @@ static int gn_launch(const eco_group_norm_plan& p, GnArgs& a, hipStream_t st) {
       threads /= 2;
     a.rows_par = (int)(threads / sl.cv);
     const long held = ceil_div(p.s, a.rows_par);          // vectors a thread
-    const dim3 grid((unsigned)(p.n * a.slabs)), block((unsigned)threads);
+    const dim3 block((unsigned)threads);
     const unsigned lds = (unsigned)((threads * VEC + 2 * sl.gb) * 4);
-    if (held <= R / 8) hipLaunchKernelGGL((gn_slab_kernel<T, VEC, R / 8>), grid, block, lds, st, a);
-    else if (held <= R / 2) hipLaunchKernelGGL((gn_slab_kernel<T, VEC, R / 2>), grid, block, lds, st, a);
-    else hipLaunchKernelGGL((gn_slab_kernel<T, VEC, R>), grid, block, lds, st, a);
-    return check_launch("eco_group_norm_forward");
+    const long most = most_workgroups(threads) / a.slabs;     // images of a launch
+    ECO_REQUIRE(most > 0, "group_norm: too many channels and positions for one launch");
+    for (long at = 0; at < p.n; at += most) {
+      const dim3 grid((unsigned)((p.n - at < most ? p.n - at : most) * a.slabs));
+      if (held <= R / 8) hipLaunchKernelGGL((gn_slab_kernel<T, VEC, R / 8>), grid, block, lds, st, a);
+      else if (held <= R / 2) hipLaunchKernelGGL((gn_slab_kernel<T, VEC, R / 2>), grid, block, lds, st, a);
+      else hipLaunchKernelGGL((gn_slab_kernel<T, VEC, R>), grid, block, lds, st, a);
+      if (int rc = check_launch("eco_group_norm_forward")) return rc;
+      a.x = (const T*)a.x + most * a.x_image;
+      a.y = (T*)a.y + most * a.y_image;
+      if (a.lengths) a.lengths += most;
+    }
+    return ECO_OK;
   }
   const long vecs = ceil_div(p.c, VEC);
   a.tiles = (int)ceil_div(vecs, kGnThreads);
@@ -559,7 +568,8 @@ static int gn_launch(const eco_group_norm_plan& p, GnArgs& a, hipStream_t st) {
   const int rows_chunk = (int)(ceil_div(ceil_div(p.s, wanted), kGnBatch / 2 * a.rows_par) * kGnBatch / 2 * a.rows_par);
   const long chunks = ceil_div(p.s, rows_chunk);
   const long results = p.n * chunks * a.tiles;
-  ECO_REQUIRE(parts <= 2147483647l && results <= 2147483647l, "group_norm: too many positions, images and channels for one launch");
+  ECO_REQUIRE(parts <= most_workgroups(kGnStatThreads) && results <= most_workgroups(kGnThreads),
+              "group_norm: too many positions, images and channels for one launch");
   hipLaunchKernelGGL((gn_stats_kernel<T, VEC>), dim3((unsigned)parts), dim3(kGnStatThreads), 0, st, a);
   if (int rc = check_launch("eco_group_norm_forward(statistics)")) return rc;
   hipLaunchKernelGGL((gn_apply_kernel<T, VEC>), dim3((unsigned)results), dim3(kGnThreads), 0, st, a, (int)chunks, rows_chunk);

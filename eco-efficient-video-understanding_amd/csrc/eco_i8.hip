@@ -157,7 +157,7 @@ struct QuantArgs {
   int lanes;     // lanes of a row (power of two up to 64)
 };
 
-// Rows of up to 64 vectors: `lanes` lanes take a row, a vector each; a wave takes ROWS sets of 64 / lanes rows, all loaded at once.
+// Rows of up to 64 vectors: `lanes` lanes take a row, a vector each; a wave takes kQuantSets sets of 64 / lanes rows, all loaded at once.
 constexpr int kQuantSets = 4;
 template <typename T, int VEC>
 __global__ __launch_bounds__(256) void quant_short_kernel(const QuantArgs a) {
@@ -255,24 +255,26 @@ __global__ __launch_bounds__(1024) void quant_long_kernel(const QuantArgs a) {
 template <typename T, int VEC>
 static int quant_launch(QuantArgs& a, hipStream_t st) {
   a.nv = (int)(a.k / VEC);
-  const unsigned m = (unsigned)a.m;
-  if (a.nv <= kWave) {
-    a.lanes = 1;
-    while (a.lanes < a.nv) a.lanes *= 2;
-    const long rows = 4l * kQuantSets * (kWave / a.lanes);           // of a workgroup
-    hipLaunchKernelGGL((quant_short_kernel<T, VEC>), dim3((unsigned)ceil_div(a.m, rows)), dim3(256), 0, st, a);
-  } else if (a.nv <= kWave * 4) {
-    hipLaunchKernelGGL((quant_row_kernel<T, VEC, 4, 64>), dim3((unsigned)ceil_div(a.m, 4)), dim3(256), 0, st, a);
-  } else if (a.nv <= 256 * 4) {
-    hipLaunchKernelGGL((quant_row_kernel<T, VEC, 4, 256>), dim3(m), dim3(256), 0, st, a);
-  } else if (a.nv <= 256 * 8) {
-    hipLaunchKernelGGL((quant_row_kernel<T, VEC, 8, 256>), dim3(m), dim3(256), 0, st, a);
-  } else if (a.nv <= 1024 * 8) {
-    hipLaunchKernelGGL((quant_row_kernel<T, VEC, 8, 1024>), dim3(m), dim3(1024), 0, st, a);
-  } else {
-    hipLaunchKernelGGL((quant_long_kernel<T, VEC>), dim3(m), dim3(1024), 0, st, a);
+  a.lanes = 1;
+  while (a.lanes < a.nv && a.lanes < kWave) a.lanes *= 2;
+  const long rows = a.nv <= kWave ? 4l * kQuantSets * (kWave / a.lanes) : a.nv <= kWave * 4 ? 4 : 1;     // of a workgroup
+  const int threads = a.nv <= 256 * 8 ? 256 : 1024;
+  const long m = a.m, most = most_workgroups(threads) * rows;                                            // rows of a launch
+  for (long at = 0; at < m; at += most) {
+    a.m = m - at < most ? m - at : most;
+    const dim3 grid((unsigned)ceil_div(a.m, rows)), block((unsigned)threads);
+    if (a.nv <= kWave) hipLaunchKernelGGL((quant_short_kernel<T, VEC>), grid, block, 0, st, a);
+    else if (a.nv <= kWave * 4) hipLaunchKernelGGL((quant_row_kernel<T, VEC, 4, 64>), grid, block, 0, st, a);
+    else if (a.nv <= 256 * 4) hipLaunchKernelGGL((quant_row_kernel<T, VEC, 4, 256>), grid, block, 0, st, a);
+    else if (a.nv <= 256 * 8) hipLaunchKernelGGL((quant_row_kernel<T, VEC, 8, 256>), grid, block, 0, st, a);
+    else if (a.nv <= 1024 * 8) hipLaunchKernelGGL((quant_row_kernel<T, VEC, 8, 1024>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((quant_long_kernel<T, VEC>), grid, block, 0, st, a);
+    if (int rc = check_launch("eco_quant_rows_forward")) return rc;
+    a.x = (const T*)a.x + most * a.ldx;
+    a.q += most * a.ldq;
+    a.scale += most;
   }
-  return check_launch("eco_quant_rows_forward");
+  return ECO_OK;
 }
 
 struct I8Args {
@@ -779,9 +781,9 @@ static int i8_launch_tile(I8Args& a, int num_cu, hipStream_t st) {
   a.tiles_m = (int)ceil_div(a.m, B);
   a.tiles_n = (int)ceil_div(a.n, B);
   const long total = ceil_div(a.m, B) * ceil_div(a.n, B) * a.ksplit;
-  ECO_REQUIRE(total <= 2147483647l, "inner_product_i8: too many tiles for one launch");
   constexpr int kLds = i8_tile_lds(B, NBUF), kPerCu = i8_tile_per_cu(B, NBUF);
   const long grid = FAST && B <= 128 && total > (long)kPerCu * num_cu ? (long)kPerCu * num_cu : total;
+  ECO_REQUIRE(grid <= most_workgroups(kI8Threads), "inner_product_i8: too many tiles for one launch");
   ECO_RAISE_DYNAMIC_LDS((i8_tile_kernel<B, NBUF, FAST, T>), "inner_product_i8");
   hipLaunchKernelGGL((i8_tile_kernel<B, NBUF, FAST, T>), dim3((unsigned)grid), dim3(kI8Threads), (unsigned)kLds, st, a);
   if (int rc = check_launch("eco_inner_product_i8_forward")) return rc;
@@ -851,7 +853,7 @@ extern "C" int eco_inner_product_i8_plan_create(int64_t m, int64_t n, int64_t k,
   ECO_REQUIRE(plan != nullptr, "inner_product_i8: null plan");
   ECO_REQUIRE(m >= 0 && n > 0 && k > 0, "inner_product_i8: bad shape");
   ECO_REQUIRE(k <= ECO_I8_MAX_K, "inner_product_i8: sums of %ld products can leave 32 bits (at most %d)", (long)k, ECO_I8_MAX_K);
-  ECO_REQUIRE(m <= 2147483647l && n <= (1l << 30), "inner_product_i8: too many rows or channels");
+  ECO_REQUIRE(m <= 2147483647l && n <= (1l << 26), "inner_product_i8: too many rows or channels");
   ECO_REQUIRE(dt == ECO_DT_F32 || dt == ECO_DT_BF16, "inner_product_i8: unknown type %d", dt);
   ECO_REQUIRE(num_cu >= 0, "inner_product_i8: negative num_cu");
   memset(plan, 0, sizeof(*plan));

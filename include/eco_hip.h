@@ -554,18 +554,18 @@ int eco_global_avgpool_fc_b_forward(const void* x, int32_t dt, const float* w, c
 #define ECO_DT_F32 0
 #define ECO_ACT_NONE 0
 #define ECO_ACT_RELU 1 /* v < 0 -> 0; a NaN stays NaN                                            */
-#define ECO_ACT_SILU 2 /* v / (1 + exp(-v))                                                      */
+#define ECO_ACT_SILU 2 /* v / (1 + exp(-v)); 0 where that is under 1e-36 (v below -87)           */
 
 /* GROUP NORM (the normalisation of eco_bn_forward with statistics of the image at hand instead of the training set's):
  *   y[i][r][ch] = act((x[i][r][ch] - mean) / sqrt(var + eps) * gamma[ch] + beta[ch])
  * with mean and (biased) variance over the c/groups channels of ch's group at every valid position of image i; statistics in
- * fp32, one rounding to dt at the store.  groups = 1 .. c. */
+ * fp32, one rounding to dt at the store.  groups = 1 .. c; s and c up to 2^30, n * groups below 2^31. */
 typedef struct eco_group_norm_plan {
   int64_t n, s;      /* images, positions of an image                                                   */
   int32_t c, groups; /* channels; groups divides c                                                      */
   int32_t dt;
   int32_t num_cu;    /* compute units that the split below is sized for                                 */
-  int32_t chunks;    /* workgroups that share an image's positions in the statistics launch             */
+  int32_t chunks;    /* > 1: workgroups that share an image's positions in the statistics launch, at most */
   int32_t reserved;
   int64_t ws_bytes;  /* device scratch of eco_group_norm_forward (0: none)                              */
 } eco_group_norm_plan;
@@ -576,9 +576,9 @@ int eco_group_norm_plan_create(int64_t n, int64_t s, int32_t c, int32_t groups, 
  * row_stride = 0: c, image_stride = 0: s*row_stride).  y may be x (same strides); otherwise they must not overlap, nor may
  * two rows of y.  lengths: device int32[n], valid positions of each image (values outside [0, s] count as 0 or s), or NULL
  * = s everywhere; positions behind an image's length are neither read nor written, and an image of length 0 is left alone.
- * gamma, beta: [c] or NULL (1 / 0).  eps >= 0.  A NaN or an infinity among a group's valid values makes that group of that image
+ * gamma, beta: [c] or NULL (1 / 0).  eps >= 0 (with 0, a group whose values are all equal becomes NaN).  A NaN or an infinity among a group's valid values makes that group of that image
  * NaN (where a fp32 formula would); other groups and images are not touched by it.
- * `workspace`: plan->ws_bytes of device scratch, its contents before and after the call unspecified.  Launches of one
+ * `workspace`: plan->ws_bytes of device scratch on a multiple of 8 bytes, its contents before and after the call unspecified.  Launches of one
  * stream may share it; calls that can run at the same time (other streams, other captured graphs) need one each. */
 int eco_group_norm_forward(const eco_group_norm_plan* plan, const void* x, int64_t x_image_stride, int64_t x_row_stride,
                            const int32_t* lengths, const float* gamma, const float* beta, float eps, int32_t act, void* y,
@@ -590,7 +590,7 @@ int eco_group_norm_forward(const eco_group_norm_plan* plan, const void* x, int64
  *              the way can move a value to the neighbouring integer, so q is the same on every build
  * q is in [-127, 127].  A row of zeros gets scale 0 and q 0.  A row with a NaN or an infinity gets scale NaN and q 0: its products
  * are NaN.  x: [m] rows of k elements, ldx elements apart (0 = k); q: [m] rows ldq bytes apart (0 = k), bytes between rows are
- * left as they were; scale: [m].  q must not overlap x. */
+ * left as they were; scale: [m].  q must not overlap x.  m below 2^31, k = 1 .. 2^30. */
 int eco_quant_rows_forward(const void* x, int32_t dt, int64_t ldx, int8_t* q, int64_t ldq, float* scale, int64_t m,
                            int64_t k, void* stream);
 
@@ -598,7 +598,8 @@ int eco_quant_rows_forward(const void* x, int32_t dt, int64_t ldx, int8_t* q, in
  * positions):
  *   y[i][j] = act(sum_l x[i][l] * w[j][l] * sx[i] * sw[j] + bias[j])
  * The sum is exact (int32; k <= ECO_I8_MAX_K keeps it so for all int8 values, -128 included), the rest is fp32 with one rounding to
- * dt (the type of y) at the store.  A folded normalisation goes into sw (scale) and bias (shift). */
+ * dt (the type of y) at the store, the factors taken from the left: the sum times sx[i] has to stay in fp32's range.  A folded
+ * normalisation goes into sw (scale) and bias (shift).  m below 2^31, n = 1 .. 2^26, k = 1 .. ECO_I8_MAX_K. */
 #define ECO_I8_MAX_K 131071
 typedef struct eco_inner_product_i8_plan {
   int64_t m;        /* rows of x and y (positions, tokens)                                               */
@@ -614,7 +615,7 @@ typedef struct eco_inner_product_i8_plan {
 int eco_inner_product_i8_plan_create(int64_t m, int64_t n, int64_t k, int32_t dt, int32_t num_cu,
                                      eco_inner_product_i8_plan* plan);
 /* x: int8 [m] rows ldx bytes apart, w: int8 [n] rows ldw bytes apart, y: [m] rows ldy elements apart (0 = dense: k, k, n);
- * rows that start on multiples of 16 bytes are read fastest.  sx: [m], sw: [n], bias: [n] or NULL.  y must not overlap an
+ * rows of x and w that start on multiples of 16 bytes, with k one too, are read fastest.  sx: [m], sw: [n], bias: [n] or NULL.  y must not overlap an
  * input.  `workspace` as in eco_group_norm_forward. */
 int eco_inner_product_i8_forward(const eco_inner_product_i8_plan* plan, const int8_t* x, int64_t ldx, const float* sx,
                                  const int8_t* w, int64_t ldw, const float* sw, const float* bias, int32_t act, void* y,

@@ -284,42 +284,25 @@ emu_f32x16 mfma_f32_32x32x16_bf16(uint4 a, uint4 b, emu_f32x16 c) {
   return d;
 }
 
-// Sum over the k groups of sixteen int8 that lanes i + R*g (A) and j + R*g (B) hold.
-static inline unsigned dot_i8(const uint4* qa, const uint4* qb, int i, int j, int R) {
-  unsigned acc = 0;
-  for (int g = 0; g < kWave / R; ++g) {
-    const signed char* pa = (const signed char*)&qa[i + R * g];
-    const signed char* pb = (const signed char*)&qb[j + R * g];
-    for (int e = 0; e < 16; ++e) acc += (unsigned)((int)pa[e] * (int)pb[e]);
-  }
-  return acc;
-}
-static inline int publish_i8(WaveState& w, uint4 a, uint4 b) {
+emu_i32x4 mfma_i32_16x16x64_i8(uint4 a, uint4 b, emu_i32x4 c) {
+  WaveState& w = my_wave();
   if (w.nlanes != kWave) {
     std::fprintf(stderr, "hip_emu: MFMA issued by a partial wave (%d lanes)\n", w.nlanes);
     std::abort();
   }
-  const int slot = wave_rendezvous_begin(w);
-  w.qa[slot][tls_cur->lane] = a;
-  w.qb[slot][tls_cur->lane] = b;
+  const int slot = wave_rendezvous_begin(w), lane = tls_cur->lane;
+  w.qa[slot][lane] = a;
+  w.qb[slot][lane] = b;
   wave_rendezvous_wait(w);
-  return slot;
-}
-
-emu_i32x16 mfma_i32_32x32x32_i8(uint4 a, uint4 b, emu_i32x16 c) {
-  WaveState& w = my_wave();
-  const int slot = publish_i8(w, a, b);
-  const int lane = tls_cur->lane;
-  for (int r = 0; r < 16; ++r)
-    c[r] = (int)((unsigned)c[r] + dot_i8(w.qa[slot], w.qb[slot], (r & 3) + 8 * (r >> 2) + 4 * (lane >> 5), lane & 31, 32));
-  return c;
-}
-
-emu_i32x4 mfma_i32_16x16x64_i8(uint4 a, uint4 b, emu_i32x4 c) {
-  WaveState& w = my_wave();
-  const int slot = publish_i8(w, a, b);
-  const int lane = tls_cur->lane;
-  for (int r = 0; r < 4; ++r) c[r] = (int)((unsigned)c[r] + dot_i8(w.qa[slot], w.qb[slot], 4 * (lane >> 4) + r, lane & 15, 16));
+  for (int r = 0; r < 4; ++r) {
+    unsigned acc = (unsigned)c[r];
+    for (int g = 0; g < 4; ++g) {
+      const signed char* pa = (const signed char*)&w.qa[slot][4 * (lane >> 4) + r + 16 * g];
+      const signed char* pb = (const signed char*)&w.qb[slot][(lane & 15) + 16 * g];
+      for (int e = 0; e < 16; ++e) acc += (unsigned)((int)pa[e] * (int)pb[e]);
+    }
+    c[r] = (int)acc;
+  }
   return c;
 }
 

@@ -64,7 +64,6 @@ static inline const char* hipGetErrorString(hipError_t) { return "emu"; }
 #define __shared__ static thread_local
 
 typedef float emu_f32x16 __attribute__((ext_vector_type(16)));
-typedef int emu_i32x16 __attribute__((ext_vector_type(16)));
 typedef int emu_i32x4 __attribute__((ext_vector_type(4)));
 
 namespace emu {
@@ -87,10 +86,8 @@ emu_f32x16 mfma_f32_32x32x2f32(float a, float b, emu_f32x16 c);
 // accumulated here in k order with one rounding each (the hardware's internal order is unspecified: compare
 // with a tolerance).
 emu_f32x16 mfma_f32_32x32x16_bf16(uint4 a, uint4 b, emu_f32x16 c);
-// v_mfma_i32_32x32x32_i8 / v_mfma_i32_16x16x64_i8: lane l holds A[i][k = 16*(l / R) + e] and B[k][j = i] as sixteen int8
-// (e = 0..15, four per dword, low byte first) with i = l % R, R = 32 or 16; C/D: 32x32 as for the f32 form, 16x16: lane l,
-// reg r holds D[4*(l>>4) + r][l & 15].  Sums wrap in 32 bits.
-emu_i32x16 mfma_i32_32x32x32_i8(uint4 a, uint4 b, emu_i32x16 c);
+// v_mfma_i32_16x16x64_i8: lane l holds A[i][k = 16*(l>>4) + e] and B[k][j = i] as sixteen int8 (e = 0..15, four per dword, low
+// byte first) with i = l & 15; C/D: lane l, reg r holds D[4*(l>>4) + r][l & 15].  Sums wrap in 32 bits.
 emu_i32x4 mfma_i32_16x16x64_i8(uint4 a, uint4 b, emu_i32x4 c);
 int readfirstlane(int v);
 void* dyn_smem();

@@ -255,6 +255,14 @@ def test_refused_calls(backend):
     assert np.array_equal(backend.host(case.dy, (case.total,)), np.full(case.total, 3.0, np.float32))   # nothing was written
 
 
+def test_refused_launches(backend):
+    """More workgroups than a launch has: refused before anything is launched (no pointer is read)."""
+    lib = backend.lib
+    for n, s, c, groups in ((1 << 24, 40000, 8, 8), (1, 32768, 1 << 24, 1 << 24)):
+        with pytest.raises(hip.EcoError, match="one launch"):
+            lib.group_norm_forward(lib.group_norm_plan(n, s, c, groups, hip.DT_F32), 4, None, None, 4, workspace=8)
+
+
 # ---- on the device: real sizes, streams, graphs ------------------------------------------------------------------------
 @pytest.mark.gpu
 @pytest.mark.parametrize("shape", [(4, 12544, 128, 32), (3, 3136, 64, 16), (1, 196, 512, 32), (2, 1568, 256, 8), (9, 1571, 210, 14),
@@ -283,6 +291,27 @@ def test_offsets_beyond_32_bits(hip_backend):
     ref, tol = formula(part.float().cpu().numpy(), 8, None, None, hip.ACT_NONE, None)
     assert (np.abs(got - ref) <= tol + UNIT[hip.DT_BF16] * np.abs(ref)).all()
     assert int((y != 0).sum()) <= n * s * c
+
+
+@pytest.mark.gpu
+def test_more_images_than_one_launch_takes(hip_backend):
+    """17 million images of one position, of every second image's length zero: 2^32 threads and more."""
+    import torch
+    n, c = (1 << 24) + 77, 8
+    x = torch.randn(n, c, device="cuda").bfloat16()
+    y = torch.full_like(x, 3.0)
+    lengths = (torch.arange(n, device="cuda") % 2).int()
+    p = hip_backend.lib.group_norm_plan(n, 1, c, 2, hip.DT_BF16)
+    assert p.ws_bytes == 0
+    hip_backend.lib.group_norm_forward(p, x.data_ptr(), None, None, y.data_ptr(), lengths=lengths.data_ptr(),
+                                       stream=torch.cuda.current_stream().cuda_stream)
+    assert bool((y[0::2] == 3.0).all())
+    z = x[1::2].double().reshape(-1, 2, c // 2)
+    mean = z.mean(2, keepdim=True)
+    rstd = 1.0 / torch.sqrt(((z - mean) ** 2).mean(2, keepdim=True) + EPS)
+    want = (z - mean) * rstd
+    tol = 16 * U32 * (z.abs() + mean.abs() + z.abs().mean(2, keepdim=True)) * rstd + UNIT[hip.DT_BF16] * want.abs()
+    assert bool(((y[1::2].double().reshape(-1, 2, c // 2) - want).abs() <= tol).all())
 
 
 @pytest.mark.gpu

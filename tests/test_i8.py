@@ -238,6 +238,15 @@ def test_product_refused_plans(backend, kw):
         backend.lib.inner_product_i8_plan(**{**dict(m=4, n=8, k=16, dt=hip.DT_F32), **kw})
 
 
+def test_product_refused_launches(backend):
+    """More channels than the plan takes; more tiles than a launch has (refused before anything is launched)."""
+    with pytest.raises(hip.EcoError, match="channels"):
+        backend.lib.inner_product_i8_plan(4, 2 ** 26 + 1, 16, hip.DT_F32)
+    p = backend.lib.inner_product_i8_plan(64 << 13, 64 << 12, 1, hip.DT_F32)
+    with pytest.raises(hip.EcoError, match="one launch"):
+        backend.lib.inner_product_i8_forward(p, 16, 16, 16, 16, None, 16, workspace=16)
+
+
 def test_product_refused_calls(backend):
     case = Product(backend, 4, 8, 16, hip.DT_F32)
     lib, p = backend.lib, backend.alloc.ptr
@@ -339,6 +348,23 @@ def test_offsets_beyond_32_bits(hip_backend):
     want_q, want_s = quant_reference(xqv.cpu().numpy())
     assert np.array_equal(torch.as_strided(q, (m, k), (ldx, 1)).cpu().numpy(), want_q)
     assert np.array_equal(s.cpu().numpy(), want_s)
+
+
+@pytest.mark.gpu
+def test_quant_more_rows_than_one_launch_takes(hip_backend):
+    """17 million rows that a workgroup each takes: 2^32 threads and more.  (Ones and a largest value per row: its integers are known.)"""
+    import torch
+    m, k = (1 << 24) + 77, 257
+    x = torch.ones(m, k, dtype=torch.bfloat16, device="cuda")
+    top = (torch.arange(m, device="cuda") % 126 + 2).bfloat16()
+    x[:, 200] = -top
+    q, s = torch.zeros(m, k, dtype=torch.int8, device="cuda"), torch.zeros(m, device="cuda")
+    hip_backend.lib.quant_rows_forward(x.data_ptr(), hip.DT_BF16, q.data_ptr(), s.data_ptr(), m, k,
+                                       stream=torch.cuda.current_stream().cuda_stream)
+    assert torch.equal(s.cpu(), top.float().cpu() / 127.0)
+    assert bool((q[:, 200] == -127).all())
+    one = torch.round(127.0 / top.double()).to(torch.int8)
+    assert bool((q[:, :200] == one[:, None]).all()) and bool((q[:, 201:] == one[:, None]).all())
 
 
 @pytest.mark.gpu
